@@ -288,6 +288,70 @@ typedef struct pa_merge_args {
 
 PA_API int pa_lse_merge(const pa_merge_args* args, pa_stream_t stream);
 
+/* ------------------------------------------------------------ paged K/V cache
+ * Serving: keys and values of many requests in a cache of pages, new tokens in
+ * chunks (down to one token), requests of any lengths.  A cache is a tensor
+ * [pages, page_size, kv_heads, D] (strides of the first three in ELEMENTS, D
+ * contiguous); row b of the block table lists request b's pages in order, so its
+ * token at position p sits at row p % page_size of page table[b][p / page_size];
+ * a slot is page * page_size + row.  No counterpart in the reference, whose
+ * attention runs over whole sequences only. */
+
+/* One step's tables from the requests' lengths, in one launch, with no host read:
+ * request b has old_lens[b] tokens in the cache and gets new_lens[b] more.
+ *   - pages it lacks are taken from free_pages, from entry *free_head on, requests in
+ *     order, and written into its row of the table; other entries are not touched;
+ *   - q_start [requests + 1]: exclusive prefix sum of the new tokens; seq_lens
+ *     [requests]: old + new;
+ *   - slot_map / positions [tokens]: slot and position of every new token, request
+ *     after request; entries past the last token get -1;
+ *   - *free_head_out = *free_head + pages taken (free_head_out != free_head);
+ *     *missing = pages that could not be had, because the free list ran out or the
+ *     table is too narrow: their table entries (inside the table) and their tokens'
+ *     slots are -1.
+ * Negative lengths count as 0; new tokens in all stay below 2^31. */
+typedef struct pa_paged_step_args {
+  int32_t requests;            /* 1 .. 16384 */
+  int32_t page_size;           /* >= 1 */
+  int32_t table_width;         /* entries per row of the table */
+  int32_t tokens;              /* capacity of slot_map / positions */
+  int32_t free_count;          /* entries of free_pages */
+  int64_t table_stride;        /* elements between rows of the table */
+  const int32_t* old_lens;
+  const int32_t* new_lens;
+  const int32_t* free_pages;
+  const int32_t* free_head;    /* [1] */
+  int32_t* block_table;        /* [requests, table_width], updated in place */
+  int32_t* q_start;
+  int32_t* seq_lens;
+  int32_t* slot_map;
+  int32_t* positions;
+  int32_t* free_head_out;      /* [1] */
+  int32_t* missing;            /* [1] */
+} pa_paged_step_args;
+
+PA_API int pa_paged_step(const pa_paged_step_args* args, pa_stream_t stream);
+
+/* Writes the K and V rows of `tokens` new tokens into their slots.  k, v: [tokens,
+ * kv_heads, D], 16-bit; slots outside [0, pages * page_size) are skipped.  Two tokens of
+ * one call must not share a slot.  Pointers 16-byte aligned, strides multiples of 8
+ * elements; k / v must not overlap the caches. */
+typedef struct pa_paged_append_args {
+  const void* k;
+  const void* v;
+  void* k_cache;
+  void* v_cache;
+  const int32_t* slot_map;
+  int32_t tokens, kv_heads, D;
+  int32_t pages, page_size;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  int64_t kc_page_stride, kc_row_stride, kc_head_stride;
+  int64_t vc_page_stride, vc_row_stride, vc_head_stride;
+} pa_paged_append_args;
+
+PA_API int pa_paged_append(const pa_paged_append_args* args, pa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

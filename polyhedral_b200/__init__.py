@@ -6,4 +6,4 @@ splits.  The reference's module names are kept: ``masks_gpu``, ``blockindex``,
 from . import masks, masks_gpu  # noqa: F401
 
 __all__ = ["masks", "masks_gpu", "blockindex", "permute", "attention", "triton_attn",
-           "merge", "split", "selector", "timing"]
+           "merge", "split", "selector", "timing", "paged"]

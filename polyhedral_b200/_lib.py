@@ -55,6 +55,26 @@ class PaMergeArgs(ctypes.Structure):
                 ("lse_bh_stride", c_i64), ("row_map2", c_vp)]
 
 
+class PaPagedStepArgs(ctypes.Structure):
+    _fields_ = [("requests", c_i32), ("page_size", c_i32), ("table_width", c_i32),
+                ("tokens", c_i32), ("free_count", c_i32), ("table_stride", c_i64),
+                ("old_lens", c_vp), ("new_lens", c_vp), ("free_pages", c_vp),
+                ("free_head", c_vp), ("block_table", c_vp), ("q_start", c_vp),
+                ("seq_lens", c_vp), ("slot_map", c_vp), ("positions", c_vp),
+                ("free_head_out", c_vp), ("missing", c_vp)]
+
+
+class PaPagedAppendArgs(ctypes.Structure):
+    _fields_ = [("k", c_vp), ("v", c_vp), ("k_cache", c_vp), ("v_cache", c_vp),
+                ("slot_map", c_vp),
+                ("tokens", c_i32), ("kv_heads", c_i32), ("D", c_i32),
+                ("pages", c_i32), ("page_size", c_i32),
+                ("k_token_stride", c_i64), ("k_head_stride", c_i64),
+                ("v_token_stride", c_i64), ("v_head_stride", c_i64),
+                ("kc_page_stride", c_i64), ("kc_row_stride", c_i64), ("kc_head_stride", c_i64),
+                ("vc_page_stride", c_i64), ("vc_row_stride", c_i64), ("vc_head_stride", c_i64)]
+
+
 # name -> (restype, argtypes); every symbol include/polyattn.h declares
 SIGNATURES = {
     "pa_last_error": (ctypes.c_char_p, []),
@@ -75,6 +95,8 @@ SIGNATURES = {
     "pa_attn_fwd_noalloc": (ctypes.c_int, [ctypes.POINTER(PaAttnArgs), c_vp]),
     "pa_attn_noalloc_status": (ctypes.c_int, [ctypes.POINTER(c_i32), c_vp]),
     "pa_lse_merge": (ctypes.c_int, [ctypes.POINTER(PaMergeArgs), c_vp]),
+    "pa_paged_step": (ctypes.c_int, [ctypes.POINTER(PaPagedStepArgs), c_vp]),
+    "pa_paged_append": (ctypes.c_int, [ctypes.POINTER(PaPagedAppendArgs), c_vp]),
 }
 
 ABI_VERSION = 8
