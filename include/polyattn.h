@@ -352,6 +352,63 @@ typedef struct pa_paged_append_args {
 
 PA_API int pa_paged_append(const pa_paged_append_args* args, pa_stream_t stream);
 
+/* Attention of every request's new tokens over its paged cache: request b's new tokens are
+ * rows q_start[b] .. q_start[b + 1] of q and o, at positions seq_lens[b] - n_b ..
+ * seq_lens[b] - 1 (n_b their number); their keys and values are in the cache already.
+ * The mask is the predicate on positions; query head a reads key head
+ * a / (heads / kv_heads).  O = sum softmax(scale q.k) v over live keys, rounded once;
+ * LSE = logsumexp of the live scaled scores (natural log); a row with no live key gets
+ * O = 0, LSE = -inf.  Keys on table entries outside [0, pages) do not count; cache rows
+ * that the mask keeps from a token, or behind a request's last token, take no part in the
+ * token's result whatever they hold.  Rows of o and lse that belong to no request are
+ * not written. */
+typedef struct pa_paged_attn_args {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  void* o;
+  float* lse;                        /* [heads, tokens] (lse_head_stride), or NULL */
+  const int32_t* block_table;        /* [requests, table_width] */
+  const int32_t* seq_lens;           /* [requests]: tokens, the new ones included */
+  const int32_t* q_start;            /* [requests + 1], ascending, ends at most at tokens */
+  int32_t requests, tokens;          /* 1 .. 65536 requests; rows of q and o */
+  int32_t heads, kv_heads, D, dtype; /* heads a multiple of kv_heads, at most 128 times;
+                                        D in {64, 128}; dtype PA_BF16 or PA_F16 */
+  int32_t pages, page_size;          /* page_size a power of two in [16, 1024] */
+  int32_t table_width;               /* table_width * page_size <= 2^24 */
+  int32_t max_new, max_len;          /* upper bounds on the new tokens / the tokens of a
+                                        request, 0 = none known: they choose how the work
+                                        is done; a request above them is served all the
+                                        same, more slowly */
+  int64_t table_stride;
+  int64_t q_token_stride, q_head_stride;
+  int64_t k_page_stride, k_row_stride, k_head_stride;
+  int64_t v_page_stride, v_row_stride, v_head_stride;
+  int64_t o_token_stride, o_head_stride;
+  int64_t lse_head_stride;
+  pa_pred pred;
+  float scale;                       /* softmax scale; <= 0 means D^-0.5 */
+} pa_paged_attn_args;
+
+/* Bytes of the plan and of one call's scratch (0: none needed) for these sizes. */
+PA_API size_t pa_paged_plan_size(const pa_paged_attn_args* args);
+PA_API size_t pa_paged_scratch_size(const pa_paged_attn_args* args);
+
+/* Builds, in `plan`, the shares of work of the forward's CTAs from seq_lens and q_start
+ * (read now, on `stream`) and the predicate.  The plan serves every forward with the same
+ * lengths, sizes and predicate -- all layers of a step -- and is only read by them, so
+ * they may run on several streams at once. */
+PA_API int pa_paged_plan(const pa_paged_attn_args* args, void* plan, size_t plan_bytes,
+                         pa_stream_t stream);
+
+/* The forward.  `scratch` (256-byte aligned) is this call's own until it has finished. */
+PA_API int pa_paged_attn(const pa_paged_attn_args* args, void* plan, size_t plan_bytes,
+                         void* scratch, size_t scratch_bytes, pa_stream_t stream);
+
+/* Status of the forwards on `plan` since it was built, synchronising `stream`: 0, or the
+ * device code of a bounded wait that ran out (PA_ERR_DEVICE). */
+PA_API int pa_paged_status(const void* plan, int32_t* status_host, pa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -75,6 +75,21 @@ class PaPagedAppendArgs(ctypes.Structure):
                 ("vc_page_stride", c_i64), ("vc_row_stride", c_i64), ("vc_head_stride", c_i64)]
 
 
+class PaPagedAttnArgs(ctypes.Structure):
+    _fields_ = [("q", c_vp), ("k_cache", c_vp), ("v_cache", c_vp), ("o", c_vp), ("lse", c_vp),
+                ("block_table", c_vp), ("seq_lens", c_vp), ("q_start", c_vp),
+                ("requests", c_i32), ("tokens", c_i32),
+                ("heads", c_i32), ("kv_heads", c_i32), ("D", c_i32), ("dtype", c_i32),
+                ("pages", c_i32), ("page_size", c_i32), ("table_width", c_i32),
+                ("max_new", c_i32), ("max_len", c_i32),
+                ("table_stride", c_i64),
+                ("q_token_stride", c_i64), ("q_head_stride", c_i64),
+                ("k_page_stride", c_i64), ("k_row_stride", c_i64), ("k_head_stride", c_i64),
+                ("v_page_stride", c_i64), ("v_row_stride", c_i64), ("v_head_stride", c_i64),
+                ("o_token_stride", c_i64), ("o_head_stride", c_i64),
+                ("lse_head_stride", c_i64), ("pred", PaPred), ("scale", c_f32)]
+
+
 # name -> (restype, argtypes); every symbol include/polyattn.h declares
 SIGNATURES = {
     "pa_last_error": (ctypes.c_char_p, []),
@@ -96,6 +111,12 @@ SIGNATURES = {
     "pa_attn_noalloc_status": (ctypes.c_int, [ctypes.POINTER(c_i32), c_vp]),
     "pa_lse_merge": (ctypes.c_int, [ctypes.POINTER(PaMergeArgs), c_vp]),
     "pa_paged_step": (ctypes.c_int, [ctypes.POINTER(PaPagedStepArgs), c_vp]),
+    "pa_paged_plan_size": (c_sz, [ctypes.POINTER(PaPagedAttnArgs)]),
+    "pa_paged_scratch_size": (c_sz, [ctypes.POINTER(PaPagedAttnArgs)]),
+    "pa_paged_plan": (ctypes.c_int, [ctypes.POINTER(PaPagedAttnArgs), c_vp, c_sz, c_vp]),
+    "pa_paged_attn": (ctypes.c_int, [ctypes.POINTER(PaPagedAttnArgs), c_vp, c_sz, c_vp, c_sz,
+                                     c_vp]),
+    "pa_paged_status": (ctypes.c_int, [c_vp, ctypes.POINTER(c_i32), c_vp]),
     "pa_paged_append": (ctypes.c_int, [ctypes.POINTER(PaPagedAppendArgs), c_vp]),
 }
 
