@@ -102,6 +102,129 @@ __device__ __forceinline__ KeyRanges key_ranges(const Pred& p, int i0, int i1, i
   return r;
 }
 
+// ------------------------------------------------------------- shares of work
+// A unit is kRows query rows (token-major, the query heads of one key head inside) of
+// one request and key head; its keys come in blocks.  The plan lines all units up,
+// request by request, key head by key head, and cuts the line into equal shares, one per
+// worker, wherever the cut falls: a unit that a cut divides is worked on by several
+// workers, whose partial results (sum, running maximum and unnormalised O of every row,
+// 32-bit) are joined by a second kernel in the order of the keys.  No counters, no order
+// that depends on timing: the same call gives the same bits.
+struct Share {
+  int b, h, t, blk;   // request, key head, unit of them, first block
+};
+
+// What the host chooses from the sizes and hints alone, alike for plan and forward.
+struct Config {
+  int unit_rows;      // query rows per unit
+  int workers;        // most shares
+  int min_share;      // blocks below which a share is not worth a worker
+  int split;          // units may be cut
+};
+
+// Blocks that a unit costs beside its own (loading q, writing o).
+constexpr int kUnitCost = 2;
+
+struct PlanView {
+  int32_t* status;
+  int32_t* meta;      // shares in use, divided units, most rows of a unit
+  Share* shares;      // [workers + 1]
+  int32_t* cuts;      // [workers] workers that begin a divided unit
+  long long* before;  // [requests + 1] cost before a request
+};
+inline __host__ size_t plan_bytes(const Config& c, int requests) {
+  return 256 + sizeof(Share) * (c.workers + 1) + 4 * (size_t)((c.workers + 1) & ~1) +
+         8 * (size_t)(requests + 1);
+}
+inline __host__ PlanView plan_view(void* p, const Config& c) {
+  char* b = static_cast<char*>(p);
+  PlanView v;
+  v.status = reinterpret_cast<int32_t*>(b);
+  v.meta = reinterpret_cast<int32_t*>(b + 64);
+  v.shares = reinterpret_cast<Share*>(b + 256);
+  v.cuts = reinterpret_cast<int32_t*>(b + 256 + sizeof(Share) * (c.workers + 1));
+  v.before = reinterpret_cast<long long*>(b + 256 + sizeof(Share) * (c.workers + 1) +
+                                          4 * (size_t)((c.workers + 1) & ~1));
+  return v;
+}
+
+// Partial result of a divided unit: worker w's piece of a unit that it does not begin
+// goes to slot 2 w, of one that it begins and does not end to slot 2 w + 1.
+template <int D>
+__host__ __device__ constexpr size_t slot_floats(int unit_rows) {
+  return (size_t)unit_rows * (D + 2);
+}
+
+// Keys of a unit whose rows sit at positions [i0, i1]: two runs of `cnt` keys a, a + step,
+// ..., of which those before `lo` are only there because a run with step 1 starts at a
+// multiple of the block.  A single position's lattice keys are listed one by one (step = the
+// modulus), so that only they are read (not if kDense).  `exact`: every listed key from
+// lo on is live for every row.
+struct Runs {
+  int a[2], cnt[2], step[2], lo[2];
+  bool exact;
+};
+template <int kBlock, bool kDense>
+__device__ __forceinline__ Runs unit_runs(const Pred& p, int i0, int i1, int len) {
+  Runs r;
+  r.step[0] = r.step[1] = 1;
+  r.exact = i0 == i1;
+  if (p.mod > 1 && i0 == i1 && !kDense) {
+    // run 0: the lattice from the band (if any) down; run 1: the band
+    const int top = min(i0, len - 1);
+    const int near = p.kind == PA_LOCAL_STRIDED ? min(max(p.p0, 0), i0 + 1) : 0;   // band's keys
+    const int far0 = p.kind == PA_FAR_STRIDED ? max(p.p0, 0) : near;
+    const long long last = min((long long)top, (long long)i0 - far0);
+    const int first = i0 >= 0 ? i0 % p.mod : 0;
+    // the last lattice key at or below `last`
+    r.a[0] = r.lo[0] = first;
+    r.step[0] = p.mod;
+    r.cnt[0] = i0 >= 0 && last >= first ? (int)((last - first) / p.mod) + 1 : 0;
+    r.lo[1] = max(i0 - near + 1, 0);
+    r.a[1] = r.lo[1] & ~(kBlock - 1);
+    r.cnt[1] = near > 0 ? max(top + 1 - r.a[1], 0) : 0;
+    return r;
+  }
+  if (p.mod > 1) r.exact = false;
+  const KeyRanges k = key_ranges(p, i0, i1, len);
+  r.lo[0] = k.a0;
+  r.lo[1] = k.a1;
+  r.a[0] = k.a0 & ~(kBlock - 1);
+  r.a[1] = k.a1 & ~(kBlock - 1);
+  r.cnt[0] = k.b0 > k.a0 ? k.b0 - r.a[0] : 0;
+  r.cnt[1] = k.b1 > k.a1 ? k.b1 - r.a[1] : 0;
+  if (r.cnt[0] > 0 && r.cnt[1] > 0 && r.a[1] < k.b0) {   // they meet in one block: one run
+    r.cnt[0] = k.b1 - r.a[0];
+    r.cnt[1] = 0;
+    r.exact = false;
+  }
+  return r;
+}
+template <int kBlock>
+__device__ __forceinline__ int run_blocks(const Runs& r) {
+  return (r.cnt[0] + kBlock - 1) / kBlock + (r.cnt[1] + kBlock - 1) / kBlock;
+}
+
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The few-rows kernel: units of 16 rows, blocks of 16 keys, a warp per share.
+constexpr int kFewRows = 16;
+constexpr int kFewBlock = 16;
+constexpr int kFewWarps = 8;
+
+// Rows of a unit of each kernel: few -- 16 rows of the request's n * group, which may begin
+// and end inside a token; see the launchers.
+int launch_few(const Params& P, bool bf16, int D, const PlanView& pv, const Config& c,
+               float* scratch, int sms, cudaStream_t stream);
+int launch_plan(const Params& P, const Config& c, const PlanView& pv, cudaStream_t stream);
+// Joins the partial results of divided units; runs behind the forward on `stream`.
+int launch_join(const Params& P, bool bf16, int D, const PlanView& pv, const Config& c,
+                const float* scratch, int sms, cudaStream_t stream);
+
 template <bool kBf16>
 __device__ __forceinline__ float2 unpack_pair(uint32_t u) {
   if constexpr (kBf16)

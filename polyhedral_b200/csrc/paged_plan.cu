@@ -1,0 +1,325 @@
+// The plan of a step's paged attention (equal shares of its key blocks) and the kernel that
+// joins the partial results of divided units.
+#include "paged.cuh"
+
+namespace pa {
+namespace paged {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+
+// Units of a request per key head, and what unit t costs in blocks.
+__device__ __forceinline__ int few_units(const Params& P, const Request& R) {
+  const long long rows = (long long)R.n * P.group;
+  return (int)((rows + kFewRows - 1) / kFewRows);
+}
+__device__ __forceinline__ int few_cost(const Params& P, const Request& R, int t) {
+  const int row0 = t * kFewRows, rows = min(R.n * P.group - row0, kFewRows);
+  const Runs r = unit_runs<kFewBlock, false>(P.pred, R.pos0 + row0 / P.group,
+                                             R.pos0 + (row0 + rows - 1) / P.group, R.len);
+  return kUnitCost + run_blocks<kFewBlock>(r);
+}
+
+// One CTA: the cost of every request, their running sum, and for each share the unit and
+// block where it begins.  A request of many units is added up, and searched, by a whole
+// warp.
+__global__ void __launch_bounds__(kPlanThreads)
+paged_plan_kernel(const __grid_constant__ Params P, Config c, PlanView pv) {
+  __shared__ long long warp_sum[kPlanThreads / 32];
+  __shared__ int s_rows, s_cuts;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int B = P.requests;
+  if (threadIdx.x == 0) {
+    s_rows = s_cuts = 0;
+    *pv.status = 0;
+  }
+  __syncthreads();
+  int rows = 0;
+  long long base = 0;
+  for (int b0 = 0; b0 < B; b0 += kPlanThreads) {
+    const int b = b0 + threadIdx.x;
+    Request R{0, 0, 0, 0};
+    if (b < B) R = get_request(P, b);
+    const int n = few_units(P, R);
+    if (n > 0) rows = max(rows, n > 1 ? kFewRows : R.n * P.group);
+    long long cost = 0;
+    if (n <= 4) {
+      for (int t = 0; t < n; ++t) cost += few_cost(P, R, t);
+    }
+    for (uint32_t big = __ballot_sync(0xffffffffu, n > 4); big; big &= big - 1) {
+      const int src = __ffs(big) - 1;
+      Request Q;
+      Q.row0 = __shfl_sync(0xffffffffu, R.row0, src);
+      Q.n = __shfl_sync(0xffffffffu, R.n, src);
+      Q.pos0 = __shfl_sync(0xffffffffu, R.pos0, src);
+      Q.len = __shfl_sync(0xffffffffu, R.len, src);
+      const int m = few_units(P, Q);
+      long long sum = 0;
+      for (int t = lane; t < m; t += 32) sum += few_cost(P, Q, t);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == src) cost = sum;
+    }
+    cost *= P.kv_heads;
+    long long x = cost;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();
+    long long before = base, all = 0;
+#pragma unroll
+    for (int i = 0; i < kPlanThreads / 32; ++i) {
+      const long long s = warp_sum[i];
+      if (i < warp) before += s;
+      all += s;
+    }
+    if (b < B) pv.before[b] = before + x - cost;
+    base += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) pv.before[B] = base;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) rows = max(rows, __shfl_xor_sync(0xffffffffu, rows, o));
+  if (lane == 0) atomicMax(&s_rows, rows);
+  __syncthreads();
+  const long long total = base;
+  long long share = (total + c.workers - 1) / c.workers;
+  if (share < c.min_share) share = c.min_share;
+  const int used = total > 0 ? (int)((total + share - 1) / share) : 0;
+
+  for (int w0 = warp * 32; w0 <= used; w0 += kPlanThreads) {
+    const int w = w0 + lane;
+    Share sh{B, 0, 0, 0};
+    long long rem = 0;
+    Request R{0, 0, 0, 0};
+    int n = 0;
+    const bool in = w < used;
+    if (in) {
+      const long long x = w * share;
+      int lo = 0, hi = B;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pv.before[mid] <= x) lo = mid; else hi = mid;
+      }
+      sh.b = lo;
+      const long long per_head = (pv.before[lo + 1] - pv.before[lo]) / P.kv_heads;
+      sh.h = (int)((x - pv.before[lo]) / per_head);
+      rem = x - pv.before[lo] - sh.h * per_head;
+      R = get_request(P, lo);
+      n = few_units(P, R);
+      if (n <= 4) {
+        int t = 0, cost = few_cost(P, R, 0);
+        while (rem >= cost && t + 1 < n) {
+          rem -= cost;
+          cost = few_cost(P, R, ++t);
+        }
+        sh.t = t;
+      }
+    }
+    for (uint32_t big = __ballot_sync(0xffffffffu, in && n > 4); big; big &= big - 1) {
+      const int src = __ffs(big) - 1;
+      Request Q;
+      Q.row0 = __shfl_sync(0xffffffffu, R.row0, src);
+      Q.n = __shfl_sync(0xffffffffu, R.n, src);
+      Q.pos0 = __shfl_sync(0xffffffffu, R.pos0, src);
+      Q.len = __shfl_sync(0xffffffffu, R.len, src);
+      long long left = __shfl_sync(0xffffffffu, rem, src);
+      const int m = few_units(P, Q);
+      int t0 = 0, found = m - 1;
+      for (; t0 < m; t0 += 32) {
+        const int cost = t0 + lane < m ? few_cost(P, Q, t0 + lane) : 0;
+        long long sum = cost;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long y = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += y;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, sum > left);
+        if (past) {
+          const int at = __ffs(past) - 1;
+          found = t0 + at;
+          left -= __shfl_sync(0xffffffffu, sum - cost, at);
+          break;
+        }
+        left -= __shfl_sync(0xffffffffu, sum, 31);
+      }
+      if (lane == src) {
+        sh.t = found;
+        rem = left;
+      }
+    }
+    if (in) {
+      // a cut inside the unit's own cost, or where units stay whole, falls on its begin --
+      // or, units staying whole, on the next unit's for all but its first cut
+      sh.blk = max((int)rem - kUnitCost, 0);
+      if (!c.split && rem > 0) {
+        sh.blk = 0;
+        if (++sh.t >= n) {
+          sh.t = 0;
+          if (++sh.h == P.kv_heads) {
+            sh.h = 0;
+            ++sh.b;
+          }
+        }
+      }
+    }
+    if (w <= used) pv.shares[w] = sh;
+  }
+  __syncthreads();
+  // the workers that begin a unit which a later one goes on with
+  for (int w = threadIdx.x; w < used; w += kPlanThreads) {
+    const Share s = pv.shares[w], e = pv.shares[w + 1];
+    const bool same = s.b == e.b && s.h == e.h && s.t == e.t;
+    if (e.blk > 0 && (!same || s.blk == 0)) pv.cuts[atomicAdd(&s_cuts, 1)] = w;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    pv.meta[0] = used;
+    pv.meta[1] = s_cuts;
+    pv.meta[2] = s_rows;
+  }
+}
+
+// One divided unit's row: O = sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i over its pieces, m
+// the largest m_i.  A warp joins a row, or, where units have many pieces, the CTA's warps
+// share them out.  (The order of `cuts` is that of an atomic counter; it decides only which
+// CTA joins which unit.)
+constexpr int kJoinWarps = 8;
+
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(kJoinWarps * 32)
+paged_join_kernel(const __grid_constant__ Params P, PlanView pv, int unit_rows,
+                  const float* __restrict__ scratch) {
+  constexpr int E = D / 32;
+  __shared__ float s_acc[kJoinWarps][D];
+  __shared__ float2 s_ml[kJoinWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int used = pv.meta[0], cuts = pv.meta[1], rows = pv.meta[2];
+  const bool many = used > kJoinWarps * cuts;   // pieces per unit, on average
+  const int items = cuts * rows;
+  const size_t slot = slot_floats<D>(unit_rows);
+  const int first = many ? blockIdx.x : blockIdx.x * kJoinWarps + warp;
+  const int step = many ? gridDim.x : gridDim.x * kJoinWarps;
+  for (int it = first; it < items; it += step) {
+    const int w0 = pv.cuts[it / rows], r = it % rows;
+    const Share e0 = pv.shares[w0 + 1];          // the unit
+    const Request R = get_request(P, e0.b);
+    const int row = e0.t * unit_rows + r;
+    if (row >= R.n * P.group) continue;          // alike for the whole CTA, where it shares a row
+    // the last worker on this unit
+    int w1 = w0 + 1;
+    while (w1 + 1 <= used) {
+      const Share e = pv.shares[w1 + 1];
+      if (!(e.b == e0.b && e.h == e0.h && e.t == e0.t)) break;
+      ++w1;
+    }
+    const int pieces = w1 - w0 + 1;
+    float m = -INFINITY, l = 0.f, acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    const int p0 = many ? warp : 0, dp = many ? kJoinWarps : 1;
+    constexpr int U = 4;
+    for (int p = p0; p < pieces; p += dp * U) {
+      float2 ml[U];
+      float x[U][E];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int q = p + u * dp;
+        ml[u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u][e] = 0.f;
+        if (q < pieces) {
+          const float* s = scratch + (size_t)(q == 0 ? 2 * w0 + 1 : 2 * (w0 + q)) * slot;
+          ml[u] = *reinterpret_cast<const float2*>(s + (size_t)unit_rows * D + 2 * r);
+          if constexpr (E == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(s + (size_t)r * D + lane * 4);
+            x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
+          } else {
+            const float2 v = *reinterpret_cast<const float2*>(s + (size_t)r * D + lane * 2);
+            x[u][0] = v.x; x[u][1] = v.y;
+          }
+        }
+      }
+      float mn = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
+      const float z = mn == -INFINITY ? 0.f : mn;
+      const float f = ex2f(m - z);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float g = ex2f(ml[u].x - z);
+        l = fmaf(g, ml[u].y, l);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(g, x[u][e], acc[e]);
+      }
+    }
+    if (many) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < E; ++e) s_acc[warp][lane * E + e] = acc[e];
+      if (lane == 0) s_ml[warp] = make_float2(m, l);
+      __syncthreads();
+      if (warp > 0) continue;
+      float mn = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kJoinWarps; ++i) mn = fmaxf(mn, s_ml[i].x);
+      const float z = mn == -INFINITY ? 0.f : mn;
+      m = mn;
+      l = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kJoinWarps; ++i) {
+        const float g = ex2f(s_ml[i].x - z);
+        l = fmaf(g, s_ml[i].y, l);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(g, s_acc[i][lane * E + e], acc[e]);
+      }
+    }
+    const int t = R.row0 + row / P.group, a = e0.h * P.group + row % P.group;
+    const float inv = l == 0.f ? 0.f : 1.f / l;   // a sum that is no number stays one
+    uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(P.o) + (long long)t * P.o_t +
+                                              (long long)a * P.o_h + lane * E);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) o[e / 2] = pack_pair<kBf16>(acc[e] * inv, acc[e + 1] * inv);
+    if (P.lse && lane == 0)
+      P.lse[a * P.lse_h + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+  }
+}
+
+}  // namespace
+
+int launch_plan(const Params& P, const Config& c, const PlanView& pv, cudaStream_t stream) {
+  paged_plan_kernel<<<1, kPlanThreads, 0, stream>>>(P, c, pv);
+  return check_launch("pa_paged_plan");
+}
+
+int launch_join(const Params& P, bool bf16, int D, const PlanView& pv, const Config& c,
+                const float* scratch, int sms, cudaStream_t stream) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(sms * 4);
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = stream;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  auto go = [&](auto kernel) -> int {
+    PA_CUDA(cudaLaunchKernelEx(&cfg, kernel, P, pv, c.unit_rows, scratch), "pa_paged_attn");
+    return PA_OK;
+  };
+  if (D == 128) return bf16 ? go(paged_join_kernel<128, true>) : go(paged_join_kernel<128, false>);
+  return bf16 ? go(paged_join_kernel<64, true>) : go(paged_join_kernel<64, false>);
+}
+
+}  // namespace paged
+}  // namespace pa

@@ -189,6 +189,7 @@ def make_plan(seq_lens, q_start, kind, p0, p1, p2, *, tokens, heads, kv_heads, h
     a.q_start = _int32("q_start", q_start, (B + 1,), dev)
     a.requests, a.tokens, a.heads, a.kv_heads = B, int(tokens), int(heads), int(kv_heads)
     a.D, a.page_size = int(head_dim), int(page_size)
+    a.table_width = max(2**24 // max(a.page_size, 1), 1)     # lengths are what seq_lens says
     a.max_new, a.max_len = int(max_new), int(max_len)
     a.pred = _lib.PaPred(int(kind), int(p0), int(p1), int(p2))
     return PagedPlan(a, seq_lens, q_start)

@@ -126,7 +126,6 @@ def test_non_finite_values_in_masked_places(bad, lens):
     for spec in ((C.WINDOW, 30, 0, 0), (C.SINKS, 30, 2, 0), (C.CAUSAL, 0, 0, 0)):
         c = C.make(*lens, 4, 2, 64, 16, BF, seed=6)
         old, new = lens
-        keep = torch.ones(0)
         for b, (x, n) in enumerate(zip(old, new)):
             t = c["block_table"][b].long()
             gone = range(2, x - 30 + 1) if spec[0] != C.CAUSAL else []
@@ -146,4 +145,6 @@ def test_non_finite_values_in_masked_places(bad, lens):
             assert not torch.isfinite(o2[last]).any()
             err = (o2.float() - o.float())[: c["tokens"]][rest.cuda()].abs().max()
             assert err <= 2.0**-7 * o.float().abs().max()
-            assert torch.equal(lse2, lse)
+            # the rows may be summed in another order now; each sum keeps the bound of
+            # paged_cases.bounds (e + 2e-5, e = 1.3e-4), so two are within twice that
+            assert (lse2 - lse)[:, : c["tokens"]].abs().max() <= 2 * (1.3e-4 + 2e-5)
