@@ -27,7 +27,8 @@ SOURCES = ["capi_util.cu", "blockindex.cu", "permute.cu", "merge.cu", "attn.cu",
            "attn_db128.cu", "attn_db128r.cu", "attn_db64.cu", "attn_db64r.cu",
            "attn_k128g.cu", "attn_k64g.cu",
            "attn_k128p.cu", "attn_k128rp.cu", "attn_k64p.cu", "attn_k64rp.cu", "attn_noalloc.cu",
-           "paged_step.cu", "paged_attn.cu", "paged_plan.cu", "paged_few.cu"]
+           "paged_step.cu", "paged_attn.cu", "paged_plan.cu", "paged_few.cu",
+           "paged_chunk64.cu", "paged_chunk128.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

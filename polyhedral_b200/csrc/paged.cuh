@@ -117,6 +117,7 @@ struct Share {
 // What the host chooses from the sizes and hints alone, alike for plan and forward.
 struct Config {
   int unit_rows;      // query rows per unit
+  int half_tokens;    // chunk kernel: tokens per half of a unit; few-rows kernel: 0
   int workers;        // most shares
   int min_share;      // blocks below which a share is not worth a worker
   int split;          // units may be cut
@@ -216,8 +217,9 @@ constexpr int kFewRows = 16;
 constexpr int kFewBlock = 16;
 constexpr int kFewWarps = 8;
 
-// Rows of a unit of each kernel: few -- 16 rows of the request's n * group, which may begin
-// and end inside a token; see the launchers.
+// Rows of a unit: few-rows kernel -- 16 of the request's n * group, which may begin and end
+// inside a token; chunk kernel -- two halves of 128, the first half_tokens * group of which
+// are whole tokens' (row r of half x: token x * half_tokens + r / group, head r % group).
 int launch_few(const Params& P, bool bf16, int D, const PlanView& pv, const Config& c,
                float* scratch, int sms, cudaStream_t stream);
 int launch_plan(const Params& P, const Config& c, const PlanView& pv, cudaStream_t stream);
@@ -241,6 +243,107 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
     __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
   }
+}
+
+// Keys of block `blk` of a unit: runs[0]'s blocks, then runs[1]'s.  Place x holds key
+// j0 + x * step; those with x in [lo, hi) are listed.
+struct BlockKeys {
+  int j0, step, lo, hi;
+};
+template <int kBlock>
+__device__ __forceinline__ BlockKeys block_keys(const Runs& r, int blk) {
+  const int n0 = (r.cnt[0] + kBlock - 1) / kBlock;
+  const int part = blk >= n0;
+  const int base = (blk - (part ? n0 : 0)) * kBlock;
+  BlockKeys k;
+  k.step = part ? r.step[1] : r.step[0];
+  k.j0 = (part ? r.a[1] : r.a[0]) + base * k.step;
+  k.lo = 0;
+  k.hi = min((part ? r.cnt[1] : r.cnt[0]) - base, kBlock);
+  if (k.step == 1) k.lo = max((part ? r.lo[1] : r.lo[0]) - k.j0, 0);
+  return k;
+}
+
+// One row (token t of q, query head h * group + g, position i) over blocks [blk0, blk1), one
+// key at a time, skipping masked keys instead of weighing their values by 0: the way out
+// when a masked key's value is not finite (0 times it is not 0).  All lanes take part;
+// lane x ends with columns [D / 32 x, D / 32 (x + 1)) of the unnormalised O.
+template <int D, bool kBf16, int kBlock>
+__device__ __noinline__ void row_by_key(const Params& P, int b, int h, int t, int g, int i,
+                                        const Runs& runs, int blk0, int blk1, float& m_out,
+                                        float& l_out, float (&acc)[D / 32]) {
+  constexpr int E = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int a = h * P.group + g;
+  const uint16_t* qp = static_cast<const uint16_t*>(P.q) + (long long)t * P.q_t +
+                       (long long)a * P.q_h + lane * E;
+  float q[E];
+#pragma unroll
+  for (int e = 0; e < E; e += 2) {
+    const float2 x = unpack_pair<kBf16>(*reinterpret_cast<const uint32_t*>(qp + e));
+    q[e] = x.x;
+    q[e + 1] = x.y;
+    acc[e] = acc[e + 1] = 0.f;
+  }
+  float m = -INFINITY, l = 0.f;
+  const int mask = (1 << P.page_shift) - 1;
+  const uint16_t* kh = static_cast<const uint16_t*>(P.k) + (long long)h * P.k_h;
+  const uint16_t* vh = static_cast<const uint16_t*>(P.v) + (long long)h * P.v_h + lane * E;
+#pragma unroll 1
+  for (int blk = blk0; blk < blk1; ++blk) {
+    const BlockKeys bk = block_keys<kBlock>(runs, blk);
+#pragma unroll 1
+    for (int x0 = 0; x0 < kBlock; x0 += 32) {        // a key per lane
+      const int x = x0 + lane, j = bk.j0 + x * bk.step;
+      bool live = x >= bk.lo && x < bk.hi && pred_live(P.pred, i, j);
+      int page = -1;
+      if (live) page = __ldg(P.table + (long long)b * P.table_stride + (j >> P.page_shift));
+      live = live && (unsigned)page < (unsigned)P.pages;
+      const long long vo = live ? page * P.v_p + (j & mask) * P.v_r : 0;
+      const uint16_t* kp = kh + (live ? page * P.k_p + (j & mask) * P.k_r : 0);
+      float s = 0.f;
+#pragma unroll 1
+      for (int d = 0; d < 32; ++d) {                  // lane d's columns of q
+        float2 y[E / 2];
+#pragma unroll
+        for (int e = 0; e < E; e += 2)
+          y[e / 2] = unpack_pair<kBf16>(*reinterpret_cast<const uint32_t*>(kp + d * E + e));
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          s = fmaf(__shfl_sync(0xffffffffu, q[e], d), y[e / 2].x, s);
+          s = fmaf(__shfl_sync(0xffffffffu, q[e + 1], d), y[e / 2].y, s);
+        }
+      }
+      s = live ? s * P.scale_log2 : -INFINITY;
+      float mn = s;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      mn = fmaxf(m, mn);
+      const float base = mn == -INFINITY ? 0.f : mn;
+      const float f = ex2f(m - base), p = live ? ex2f(s - base) : 0.f;
+      m = mn;
+      float sum = p;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      l = l * f + sum;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= f;
+#pragma unroll 1
+      for (uint32_t todo = __ballot_sync(0xffffffffu, live); todo; todo &= todo - 1) {
+        const int y = __ffs(todo) - 1;
+        const float py = __shfl_sync(0xffffffffu, p, y);
+        const uint16_t* vp = vh + __shfl_sync(0xffffffffu, vo, y);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 z = unpack_pair<kBf16>(*reinterpret_cast<const uint32_t*>(vp + e));
+          acc[e] = fmaf(py, z.x, acc[e]);
+          acc[e + 1] = fmaf(py, z.y, acc[e + 1]);
+        }
+      }
+    }
+  }
+  m_out = m;
+  l_out = l;
 }
 
 }  // namespace paged

@@ -1,5 +1,6 @@
 // Attention over a paged K/V cache: argument checks, the plan and the C entry points.
-#include "paged.cuh"
+#include <mutex>
+#include "paged_chunk.cuh"
 
 namespace pa {
 namespace paged {
@@ -88,13 +89,92 @@ int sm_count(int* sms) {
 // Kernel and shares for these sizes and hints.
 Config choose(const pa_paged_attn_args* a, int sms) {
   Config c;
-  c.unit_rows = kFewRows;
-  c.workers = sms * kFewWarps;
-  c.min_share = 4 + kUnitCost;
+  const int group = a->heads / a->kv_heads;
+  const long long most = a->max_new > 0 && a->max_new < a->tokens ? a->max_new : a->tokens;
+  if (most * group <= kFewRows) {
+    c.unit_rows = kFewRows;
+    c.half_tokens = 0;
+    c.workers = sms * kFewWarps;
+    c.min_share = 4 + kUnitCost;
+  } else {
+    c.unit_rows = 256;
+    c.half_tokens = 128 / group;
+    c.workers = sms;
+    c.min_share = 2 + kUnitCost;
+  }
   // a request's keys that fit two shares are read by one warp sooner than by several
   // and the join behind them
   c.split = !(a->max_len > 0 && a->max_len <= 128);
   return c;
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                             const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                             CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(p);
+  });
+  return fn;
+}
+
+// 16-bit tensor (D, n1, n2, n3) by element strides s1..s3, in boxes of 64 x b1 x 1 x b3, 128-byte
+// swizzle, zeros outside.
+int make_map(CUtensorMap* m, const void* base, int dtype, int D, const long long (&n)[3],
+             const long long (&s)[3], int b1, int b3, const char* name) {
+  EncodeFn enc = encode_fn();
+  if (!enc) return fail(PA_ERR_CUDA, "pa_paged_attn: cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[4] = {(cuuint64_t)D, 0, 0, 0}, strides[3];
+  const cuuint32_t box[4] = {64, (cuuint32_t)b1, 1, (cuuint32_t)b3}, one[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 3; ++i) {
+    dims[i + 1] = (cuuint64_t)n[i];
+    strides[i] = n[i] > 1 ? (cuuint64_t)s[i] * 2 : (cuuint64_t)D * 2;   // unused where there is one
+  }
+  const CUresult r =
+      enc(m, dtype == PA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+          const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(PA_ERR_ARG, "pa_paged_attn: tensor map for %s rejected (CUresult %d): check its strides",
+                name, (int)r);
+  return PA_OK;
+}
+
+int launch_chunk(const pa_paged_attn_args* a, const Params& P, const Config& c, const PlanView& pv,
+                 float* scratch, int sms, cudaStream_t stream) {
+  CUtensorMap tq, tk, tv;
+  int rc;
+  ChunkParams C;
+  C.p = P;
+  C.tb = c.half_tokens;
+  C.seg = a->page_size < 128 ? a->page_size : 128;
+  C.nseg = 128 / C.seg;
+  if ((rc = make_map(&tq, a->q, a->dtype, a->D, {P.group, a->kv_heads, a->tokens},
+                     {a->q_head_stride, a->q_head_stride * P.group, a->q_token_stride}, P.group, C.tb,
+                     "q")))
+    return rc;
+  if ((rc = make_map(&tk, a->k_cache, a->dtype, a->D, {a->page_size, a->kv_heads, a->pages},
+                     {a->k_row_stride, a->k_head_stride, a->k_page_stride}, C.seg, 1, "k_cache")))
+    return rc;
+  if ((rc = make_map(&tv, a->v_cache, a->dtype, a->D, {a->page_size, a->kv_heads, a->pages},
+                     {a->v_row_stride, a->v_head_stride, a->v_page_stride}, C.seg, 1, "v_cache")))
+    return rc;
+  const uint32_t fmt = a->dtype == PA_BF16 ? 1u : 0u;
+  C.idesc_qk = make_idesc_f16(fmt, 128, 128, 0, 0);
+  C.idesc_pv = make_idesc_f16(fmt, 128, a->D, 0, 1);
+  C.err.word = pv.status;
+  C.err.epoch = 0;
+  C.err.limit_ns = kWaitLimitNs;
+  return a->D == 128 ? launch_chunk_d128(tq, tk, tv, C, fmt != 0, pv, scratch, sms, stream)
+                     : launch_chunk_d64(tq, tk, tv, C, fmt != 0, pv, scratch, sms, stream);
 }
 
 size_t scratch_bytes_of(const pa_paged_attn_args* a, const Config& c) {
@@ -161,7 +241,9 @@ extern "C" int pa_paged_attn(const pa_paged_attn_args* a, void* plan, size_t pla
   const PlanView pv = plan_view(plan, c);
   const cudaStream_t s = (cudaStream_t)stream;
   const bool bf = a->dtype == PA_BF16;
-  if ((rc = launch_few(P, bf, a->D, pv, c, static_cast<float*>(scratch), sms, s))) return rc;
+  rc = c.half_tokens ? launch_chunk(a, P, c, pv, static_cast<float*>(scratch), sms, s)
+                     : launch_few(P, bf, a->D, pv, c, static_cast<float*>(scratch), sms, s);
+  if (rc) return rc;
   return c.split ? launch_join(P, bf, a->D, pv, c, static_cast<const float*>(scratch), sms, s)
                  : PA_OK;
 }

@@ -58,91 +58,13 @@ struct Few {
   static constexpr int kBytes = kMetaOff + kFewWarps * kStages * 4;
 };
 
-// A piece of a unit: its blocks [blk0, blk1) of n, and where its rows go.
+// A piece of a unit: its blocks [blk0, blk1), and where its rows go.
 struct Piece {
   Request R;
   Runs runs;
   int b, h, row0, rows, blk0, blk1;
   float* slot;        // partial result, or null: o and lse
 };
-
-// Key of a block's place x, for block `blk` of the unit: runs[0]'s blocks, then runs[1]'s.
-struct BlockKeys {
-  int j0, step, lo, hi;   // keys j0 + x * step, those with x in [lo, hi) listed
-};
-__device__ __forceinline__ BlockKeys block_keys(const Runs& r, int blk) {
-  const int n0 = (r.cnt[0] + kFewBlock - 1) / kFewBlock;
-  const int part = blk >= n0;
-  const int base = (blk - (part ? n0 : 0)) * kFewBlock;
-  BlockKeys k;
-  k.step = part ? r.step[1] : r.step[0];
-  k.j0 = (part ? r.a[1] : r.a[0]) + base * k.step;
-  k.lo = 0;
-  k.hi = min((part ? r.cnt[1] : r.cnt[0]) - base, kFewBlock);
-  if (k.step == 1) k.lo = max((part ? r.lo[1] : r.lo[0]) - k.j0, 0);
-  return k;
-}
-
-// One row over the piece's keys, one key at a time, skipping masked keys instead of
-// weighing their values by 0: the way out when a masked key's value is not finite
-// (0 times it is not 0).  All lanes take part; lane x holds columns [D / 32 x, D / 32 (x + 1)).
-template <int D, bool kBf16>
-__device__ __noinline__ void row_by_key(const Params& P, const Piece& c, int row,
-                                        float& m_out, float& l_out, float (&acc)[D / 32]) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int t = row / P.group, a = c.h * P.group + row % P.group;
-  const int i = c.R.pos0 + t;
-  const uint16_t* qp = static_cast<const uint16_t*>(P.q) + (long long)(c.R.row0 + t) * P.q_t +
-                       a * P.q_h + lane * E;
-  float q[E];
-#pragma unroll
-  for (int e = 0; e < E; e += 2) {
-    const float2 x = unpack_pair<kBf16>(*reinterpret_cast<const uint32_t*>(qp + e));
-    q[e] = x.x;
-    q[e + 1] = x.y;
-    acc[e] = acc[e + 1] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  const int mask = (1 << P.page_shift) - 1;
-#pragma unroll 1
-  for (int blk = c.blk0; blk < c.blk1; ++blk) {
-    const BlockKeys bk = block_keys(c.runs, blk);
-#pragma unroll 1
-    for (int x = bk.lo; x < bk.hi; ++x) {
-      const int j = bk.j0 + x * bk.step;
-      if (!pred_live(P.pred, i, j)) continue;
-      const int page = __ldg(P.table + c.b * P.table_stride + (j >> P.page_shift));
-      if ((unsigned)page >= (unsigned)P.pages) continue;
-      const uint16_t* kp = static_cast<const uint16_t*>(P.k) + page * P.k_p + (j & mask) * P.k_r +
-                           c.h * P.k_h + lane * E;
-      const uint16_t* vp = static_cast<const uint16_t*>(P.v) + page * P.v_p + (j & mask) * P.v_r +
-                           c.h * P.v_h + lane * E;
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const float2 y = unpack_pair<kBf16>(*reinterpret_cast<const uint32_t*>(kp + e));
-        s = fmaf(q[e], y.x, fmaf(q[e + 1], y.y, s));
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      s *= P.scale_log2;
-      const float mn = fmaxf(m, s);
-      const float base = mn == -INFINITY ? 0.f : mn;
-      const float f = ex2f(m - base), p = ex2f(s - base);
-      m = mn;
-      l = l * f + p;
-#pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const float2 y = unpack_pair<kBf16>(*reinterpret_cast<const uint32_t*>(vp + e));
-        acc[e] = acc[e] * f + p * y.x;
-        acc[e + 1] = acc[e + 1] * f + p * y.y;
-      }
-    }
-  }
-  m_out = m;
-  l_out = l;
-}
 
 template <int D, bool kBf16>
 __device__ __noinline__ void piece_by_key(const Params& P, const Piece& c) {
@@ -152,7 +74,8 @@ __device__ __noinline__ void piece_by_key(const Params& P, const Piece& c) {
   for (int r = 0; r < c.rows; ++r) {
     float m, l, acc[E];
     const int row = c.row0 + r;
-    row_by_key<D, kBf16>(P, c, row, m, l, acc);
+    row_by_key<D, kBf16, kFewBlock>(P, c.b, c.h, c.R.row0 + row / P.group, row % P.group,
+                                   c.R.pos0 + row / P.group, c.runs, c.blk0, c.blk1, m, l, acc);
     if (c.slot) {
 #pragma unroll
       for (int e = 0; e < E; ++e) c.slot[r * D + lane * E + e] = acc[e];
@@ -252,7 +175,7 @@ paged_few_kernel(const __grid_constant__ Params P, const Share* __restrict__ sha
     // page of place (lane & 15) of block blk, read a block ahead of its rows
     auto page_of = [&](int blk) -> int {
       if (blk >= c.blk1) return -1;
-      const BlockKeys k = block_keys(c.runs, blk);
+      const BlockKeys k = block_keys<kFewBlock>(c.runs, blk);
       const int x = lane & 15;
       if (x < k.lo || x >= k.hi) return -1;
       return __ldg(trow + ((k.j0 + x * k.step) >> P.page_shift));
@@ -261,7 +184,7 @@ paged_few_kernel(const __grid_constant__ Params P, const Share* __restrict__ sha
     auto load = [&](int blk, int page) {
       if (blk < c.blk1) {
         const int st = (blk - c.blk0) % S;
-        const BlockKeys k = block_keys(c.runs, blk);
+        const BlockKeys k = block_keys<kFewBlock>(c.runs, blk);
         const int j = k.j0 + (lane & 15) * k.step;
         const bool ok = (unsigned)page < (unsigned)P.pages;
         const uint32_t live = __ballot_sync(0xffffffffu, ok) & 0xffffu;
@@ -310,7 +233,7 @@ paged_few_kernel(const __grid_constant__ Params P, const Share* __restrict__ sha
       const int st = (blk - c.blk0) % S;
       const uint32_t sk = ring + st * 2 * F::kTile, sv = sk + F::kTile;
       const uint32_t live = s_live[st];
-      const BlockKeys k = block_keys(c.runs, blk);
+      const BlockKeys k = block_keys<kFewBlock>(c.runs, blk);
 
       float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
       {

@@ -9,15 +9,24 @@ namespace {
 constexpr int kPlanThreads = 1024;
 
 // Units of a request per key head, and what unit t costs in blocks.
-__device__ __forceinline__ int few_units(const Params& P, const Request& R) {
-  const long long rows = (long long)R.n * P.group;
-  return (int)((rows + kFewRows - 1) / kFewRows);
+__device__ __forceinline__ int unit_count(const Params& P, const Config& c, const Request& R) {
+  if (c.half_tokens) return (R.n + 2 * c.half_tokens - 1) / (2 * c.half_tokens);
+  return (R.n * P.group + kFewRows - 1) / kFewRows;
 }
-__device__ __forceinline__ int few_cost(const Params& P, const Request& R, int t) {
+__device__ __forceinline__ int unit_cost(const Params& P, const Config& c, const Request& R, int t) {
+  if (c.half_tokens) {
+    const int t0 = t * 2 * c.half_tokens;
+    return kUnitCost + run_blocks<128>(unit_runs<128, true>(
+                           P.pred, R.pos0 + t0, R.pos0 + min(R.n, t0 + 2 * c.half_tokens) - 1, R.len));
+  }
   const int row0 = t * kFewRows, rows = min(R.n * P.group - row0, kFewRows);
-  const Runs r = unit_runs<kFewBlock, false>(P.pred, R.pos0 + row0 / P.group,
-                                             R.pos0 + (row0 + rows - 1) / P.group, R.len);
-  return kUnitCost + run_blocks<kFewBlock>(r);
+  return kUnitCost + run_blocks<kFewBlock>(unit_runs<kFewBlock, false>(
+                         P.pred, R.pos0 + row0 / P.group, R.pos0 + (row0 + rows - 1) / P.group, R.len));
+}
+// Rows of a request's largest unit that hold a token.
+__device__ __forceinline__ int unit_rows_used(const Params& P, const Config& c, const Request& R) {
+  if (c.half_tokens) return R.n > c.half_tokens ? 256 : R.n * P.group;
+  return min(R.n * P.group, kFewRows);
 }
 
 // One CTA: the cost of every request, their running sum, and for each share the unit and
@@ -40,11 +49,11 @@ paged_plan_kernel(const __grid_constant__ Params P, Config c, PlanView pv) {
     const int b = b0 + threadIdx.x;
     Request R{0, 0, 0, 0};
     if (b < B) R = get_request(P, b);
-    const int n = few_units(P, R);
-    if (n > 0) rows = max(rows, n > 1 ? kFewRows : R.n * P.group);
+    const int n = unit_count(P, c, R);
+    rows = max(rows, unit_rows_used(P, c, R));
     long long cost = 0;
     if (n <= 4) {
-      for (int t = 0; t < n; ++t) cost += few_cost(P, R, t);
+      for (int t = 0; t < n; ++t) cost += unit_cost(P, c, R, t);
     }
     for (uint32_t big = __ballot_sync(0xffffffffu, n > 4); big; big &= big - 1) {
       const int src = __ffs(big) - 1;
@@ -53,9 +62,9 @@ paged_plan_kernel(const __grid_constant__ Params P, Config c, PlanView pv) {
       Q.n = __shfl_sync(0xffffffffu, R.n, src);
       Q.pos0 = __shfl_sync(0xffffffffu, R.pos0, src);
       Q.len = __shfl_sync(0xffffffffu, R.len, src);
-      const int m = few_units(P, Q);
+      const int m = unit_count(P, c, Q);
       long long sum = 0;
-      for (int t = lane; t < m; t += 32) sum += few_cost(P, Q, t);
+      for (int t = lane; t < m; t += 32) sum += unit_cost(P, c, Q, t);
 #pragma unroll
       for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (lane == src) cost = sum;
@@ -109,12 +118,12 @@ paged_plan_kernel(const __grid_constant__ Params P, Config c, PlanView pv) {
       sh.h = (int)((x - pv.before[lo]) / per_head);
       rem = x - pv.before[lo] - sh.h * per_head;
       R = get_request(P, lo);
-      n = few_units(P, R);
+      n = unit_count(P, c, R);
       if (n <= 4) {
-        int t = 0, cost = few_cost(P, R, 0);
+        int t = 0, cost = unit_cost(P, c, R, 0);
         while (rem >= cost && t + 1 < n) {
           rem -= cost;
-          cost = few_cost(P, R, ++t);
+          cost = unit_cost(P, c, R, ++t);
         }
         sh.t = t;
       }
@@ -127,10 +136,10 @@ paged_plan_kernel(const __grid_constant__ Params P, Config c, PlanView pv) {
       Q.pos0 = __shfl_sync(0xffffffffu, R.pos0, src);
       Q.len = __shfl_sync(0xffffffffu, R.len, src);
       long long left = __shfl_sync(0xffffffffu, rem, src);
-      const int m = few_units(P, Q);
+      const int m = unit_count(P, c, Q);
       int t0 = 0, found = m - 1;
       for (; t0 < m; t0 += 32) {
-        const int cost = t0 + lane < m ? few_cost(P, Q, t0 + lane) : 0;
+        const int cost = t0 + lane < m ? unit_cost(P, c, Q, t0 + lane) : 0;
         long long sum = cost;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -191,7 +200,7 @@ constexpr int kJoinWarps = 8;
 
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kJoinWarps * 32)
-paged_join_kernel(const __grid_constant__ Params P, PlanView pv, int unit_rows,
+paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
                   const float* __restrict__ scratch) {
   constexpr int E = D / 32;
   __shared__ float s_acc[kJoinWarps][D];
@@ -201,6 +210,7 @@ paged_join_kernel(const __grid_constant__ Params P, PlanView pv, int unit_rows,
   const int used = pv.meta[0], cuts = pv.meta[1], rows = pv.meta[2];
   const bool many = used > kJoinWarps * cuts;   // pieces per unit, on average
   const int items = cuts * rows;
+  const int unit_rows = c.unit_rows;
   const size_t slot = slot_floats<D>(unit_rows);
   const int first = many ? blockIdx.x : blockIdx.x * kJoinWarps + warp;
   const int step = many ? gridDim.x : gridDim.x * kJoinWarps;
@@ -208,8 +218,22 @@ paged_join_kernel(const __grid_constant__ Params P, PlanView pv, int unit_rows,
     const int w0 = pv.cuts[it / rows], r = it % rows;
     const Share e0 = pv.shares[w0 + 1];          // the unit
     const Request R = get_request(P, e0.b);
-    const int row = e0.t * unit_rows + r;
-    if (row >= R.n * P.group) continue;          // alike for the whole CTA, where it shares a row
+    int tok, g;                                  // token of the request, head of the group
+    bool there;
+    if (c.half_tokens) {
+      const int x = r & 127;
+      tok = x / P.group;
+      g = x - tok * P.group;
+      there = tok < c.half_tokens;
+      tok += (e0.t * 2 + (r >> 7)) * c.half_tokens;
+      there = there && tok < R.n;
+    } else {
+      const int row = e0.t * kFewRows + r;
+      tok = row / P.group;
+      g = row - tok * P.group;
+      there = tok < R.n;
+    }
+    if (!there) continue;                        // alike for the whole CTA, where it shares a row
     // the last worker on this unit
     int w1 = w0 + 1;
     while (w1 + 1 <= used) {
@@ -284,7 +308,7 @@ paged_join_kernel(const __grid_constant__ Params P, PlanView pv, int unit_rows,
         for (int e = 0; e < E; ++e) acc[e] = fmaf(g, s_acc[i][lane * E + e], acc[e]);
       }
     }
-    const int t = R.row0 + row / P.group, a = e0.h * P.group + row % P.group;
+    const int t = R.row0 + tok, a = e0.h * P.group + g;
     const float inv = l == 0.f ? 0.f : 1.f / l;   // a sum that is no number stays one
     uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(P.o) + (long long)t * P.o_t +
                                               (long long)a * P.o_h + lane * E);
@@ -314,7 +338,7 @@ int launch_join(const Params& P, bool bf16, int D, const PlanView& pv, const Con
   cfg.attrs = at;
   cfg.numAttrs = 1;
   auto go = [&](auto kernel) -> int {
-    PA_CUDA(cudaLaunchKernelEx(&cfg, kernel, P, pv, c.unit_rows, scratch), "pa_paged_attn");
+    PA_CUDA(cudaLaunchKernelEx(&cfg, kernel, P, c, pv, scratch), "pa_paged_attn");
     return PA_OK;
   };
   if (D == 128) return bf16 ? go(paged_join_kernel<128, true>) : go(paged_join_kernel<128, false>);
