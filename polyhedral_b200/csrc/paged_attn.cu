@@ -76,7 +76,12 @@ int make_params(const pa_paged_attn_args* a, Params* P, const char* who) {
   P->page_shift = a->page_size > 0 ? __builtin_ctz(a->page_size) : 0;
   const float scale = a->scale > 0.f ? a->scale : 1.0f / sqrtf((float)a->D);
   P->scale_log2 = scale * 1.4426950408889634f;
-  return make_pred(&a->pred, &P->pred, who);
+  // positions stay below 2^24, so larger widths mean the same and would overflow sums
+  pa_pred pr = a->pred;
+  pr.p0 = pr.p0 < (1 << 25) ? pr.p0 : 1 << 25;
+  pr.p1 = pr.p1 < (1 << 25) ? pr.p1 : 1 << 25;
+  pr.p2 = pr.p2 < (1 << 25) ? pr.p2 : 1 << 25;
+  return make_pred(&pr, &P->pred, who);
 }
 
 int sm_count(int* sms) {
@@ -167,6 +172,7 @@ int launch_chunk(const pa_paged_attn_args* a, const Params& P, const Config& c, 
   if ((rc = make_map(&tv, a->v_cache, a->dtype, a->D, {a->page_size, a->kv_heads, a->pages},
                      {a->v_row_stride, a->v_head_stride, a->v_page_stride}, C.seg, 1, "v_cache")))
     return rc;
+  C.o32 = aligned(a->o, 32) && a->o_token_stride % 16 == 0 && a->o_head_stride % 16 == 0;
   const uint32_t fmt = a->dtype == PA_BF16 ? 1u : 0u;
   C.idesc_qk = make_idesc_f16(fmt, 128, 128, 0, 0);
   C.idesc_pv = make_idesc_f16(fmt, 128, a->D, 0, 1);

@@ -12,7 +12,7 @@
 //   warp 9       matrix products: S = Q K^T and O += P V of each half in turn, so that one
 //                half's softmax runs under the other half's products;
 //   warps 0-3    softmax of half 0 (a thread per row), warps 4-7 of half 1: S comes from
-//                and P (16-bit) goes to tensor memory, two 64-key parts, the product of the
+//                and P (16-bit) goes to tensor memory in two 64-key parts, the product of the
 //                first running while the second is still exponentiated; the running
 //                maximum is moved, and O rescaled, only when it has grown by more than 2^8;
 //   warps 10-11  complete the third warpgroup, so that registers can move to the softmax.
@@ -39,12 +39,23 @@ struct ChunkParams {
   Params p;
   int tb;                 // tokens per half: 128 / group
   int seg, nseg;          // rows of a page's box, boxes per super-tile
+  int o32;                // rows of o are 32-byte aligned
   uint32_t idesc_qk, idesc_pv;
   ErrSink err;
 };
 
+// What decides, for one half of a unit, the kind of the super-tile at key kb: some row sees
+// some of it when kb <= i_hi and (kb >= live_min or kb < sink_end); every row sees all of it
+// when full_min <= kb <= full_max and all its boxes have keys.
+struct __align__(16) HalfTiles {
+  int i_hi, live_min, full_min, full_max;
+};
+
 // A piece of a unit, handed from the copying warp to the others.
-struct ChunkUnit {
+struct __align__(16) ChunkUnit {
+  HalfTiles half[2];
+  int a0, a1, n0, sink_end;       // super-tile blk: a0 + 128 blk, from n0 on a1 + 128 (blk - n0)
+  const int32_t* table;           // the request's row of the block table
   int b, h;               // b < 0: no more
   int row0, n;            // first token's row of q, tokens of the unit
   int pos0, len;          // its position; tokens of the request
@@ -56,10 +67,9 @@ struct ChunkUnit {
 template <int D>
 struct ChunkSmem {
   static constexpr int kTile = 128 * D * 2;
-  static constexpr int kSlots = D == 128 ? 4 : 8;
+  static constexpr int kSlots = D == 128 ? 5 : 10;
   static constexpr int kKVOff = 2 * kTile;
-  static constexpr int kEpiOff = kKVOff + kSlots * kTile;            // 8 warps x 32 rows x 128 bytes
-  static constexpr int kBarOff = kEpiOff + 8 * 32 * 128;
+  static constexpr int kBarOff = kKVOff + kSlots * kTile;
   // q_full[2] q_empty[2] s_full[2] pa_full[2] pb_full[2] o_full[2] drain unit_full[2]
   // unit_empty[2] kv_full[S] kv_empty[S]
   static constexpr int kNumBars = 17 + 2 * kSlots;
@@ -69,6 +79,57 @@ struct ChunkSmem {
   static constexpr int kAlloc = kBytes + 1024;
   static_assert(kAlloc <= 232448, "shared memory of one CTA");
 };
+
+__device__ __forceinline__ HalfTiles half_tiles(const Pred& p, int i_lo, int i_hi, int len) {
+  const bool window = p.kind == PA_WINDOW || p.kind == PA_SINKS;
+  HalfTiles t;
+  t.i_hi = i_hi;
+  t.live_min = window ? i_lo - p.p0 - 126 : INT32_MIN;
+  t.full_min = window ? i_hi - p.p0 + 1 : p.kind == PA_CAUSAL ? 0 : INT32_MAX;
+  t.full_max = min(i_lo - 127, len - 128);
+  return t;
+}
+__device__ __forceinline__ bool tile_live(const HalfTiles& t, int kb, int sink_end) {
+  return kb <= t.i_hi && (kb >= t.live_min || kb < sink_end);
+}
+// 16 bytes of shared memory, read where it is written and kept no longer: the softmax
+// threads have no register to spare, and a spilled one costs a trip to L2 (their local
+// memory does not fit what shared memory leaves of L1).
+__device__ __forceinline__ int4 lds4(const void* p) {
+  int4 v;
+  asm volatile("ld.shared.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(smem_u32(p)));
+  return v;
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32"
+      " {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+// 32 bytes to global memory, at once where the address is a multiple of 32.
+__device__ __forceinline__ void st32(void* p, bool whole, uint32_t a, uint32_t b, uint32_t c,
+                                     uint32_t d, uint32_t e, uint32_t f, uint32_t g, uint32_t h) {
+  if (whole) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(p), "r"(a), "r"(b), "r"(c), "r"(d), "r"(e), "r"(f), "r"(g), "r"(h) : "memory");
+  } else {
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(a, b, c, d);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(e, f, g, h);
+  }
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(r));
+  return r != 0;
+}
 
 // 2^x for two values on the FMA and integer pipes: j = rint(x) by adding 1.5 * 2^23, 2^(x - j)
 // by a degree-4 polynomial fitted for least maximum relative error on [-1/2, 1/2] (2.7e-6 in
@@ -90,10 +151,14 @@ __device__ __forceinline__ void exp2_poly(float x0, float x1, float& y0, float& 
   attn::fma2v(y0, y1, p0, p1, s0, s1, 0.0f, 0.0f);
 }
 
-// Pairs, of the 16 of each 32 columns, whose exponentials run on the FMA pipe.
+// Pairs, of the 16 of each 32 columns, whose exponentials run on the FMA pipe.  At D = 64
+// the products take half as long and the exponential unit is what both halves wait for: 4
+// of 16 pairs moved, 24 ragged requests took 109 us instead of 114.  At D = 128 they leave
+// the issue slots too few: 2 of 16 moved, 4096 new tokens over 16384 took 1086 us instead
+// of 1076, 4 of 16 1127 us.
 template <int D>
 __device__ __forceinline__ constexpr bool on_fma(int pair) {
-  return false;
+  return D == 64 && (pair & 3) == 3;
 }
 
 template <int D, bool kBf16>
@@ -129,7 +194,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   int* s_slow = reinterpret_cast<int*>(smem + SM::kMiscOff + 8);   // warps going key by key
   ChunkUnit* s_unit = reinterpret_cast<ChunkUnit*>(smem + SM::kUnitOff);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const ErrSink& err = C.err;
   // A bounded wait (mbar_wait); the time in which a warp goes key by key does not count.
   auto wait_bar = [&](uint64_t* bar, uint32_t parity, int32_t code) -> bool {
@@ -232,6 +297,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           u.blk0 = fresh ? min(first.blk, nblk) : 0;
           u.blk1 = last ? min(end.blk, nblk) : nblk;
           u.slot = fresh && first.blk > 0 ? 2 * w : last ? 2 * w + 1 : -1;
+          for (int x = 0; x < 2; ++x)
+            u.half[x] = half_tiles(P.pred, u.pos0 + x * C.tb,
+                                   u.pos0 + min(u.n, (x + 1) * C.tb) - 1, u.len);
+          u.a0 = u.runs.a[0];
+          u.a1 = u.runs.a[1];
+          u.n0 = (u.runs.cnt[0] + 127) >> 7;
+          u.sink_end = P.pred.kind == PA_SINKS ? P.pred.p1 : 0;
+          u.table = P.table + (long long)u.b * P.table_stride;
           fresh = false;
           ++at.t;
           break;
@@ -328,87 +401,122 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       }
     } else if (warp == kChunkMmaWarp) {
       // ------------------------------------------------------------ matrix products
-      if (lane == 0) {
-        uint32_t ring = 0, kv_c = 0, tp[2] = {0, 0}, tq[2] = {0, 0};
-        bool ok = true;
-        const uint32_t sQa = smem_u32(sQ), sKVa = smem_u32(sKV);
-        const uint64_t q_desc[2] = {smem_desc_sw128(sQa, 16), smem_desc_sw128(sQa + SM::kTile, 16)};
-        auto wait_kv = [&](uint32_t& slot) -> bool {
-          slot = kv_c % NS;
-          const bool r = wait_bar(&kv_full[slot], (kv_c / NS) & 1, DEV_TIMEOUT_KV);
-          ++kv_c;
-          tc_fence_after();
-          return r;
-        };
-        auto issue_s = [&](int h, uint32_t kslot) {
-          const uint64_t kd = smem_desc_sw128(sKVa + kslot * SM::kTile, 16);
+      // The whole warp runs this code, one elected lane issues: then every address is the
+      // same in all lanes for the compiler too and stays in uniform registers.  (With
+      // one lane in the whole branch, a product took 97 cycles to issue where the tensor
+      // cores take 64: 4096 new tokens over 16384 were 1215 us.)
+      const bool leader = elect_one();
+      uint32_t ring = 0, kv_c = 0, tp[2] = {0, 0}, tq[2] = {0, 0};
+      bool ok = true;
+      const uint32_t sQa = smem_u32(sQ), sKVa = smem_u32(sKV);
+      auto wait_all = [&](uint64_t* bar, uint32_t parity, int32_t code) -> bool {
+        const bool r = __all_sync(0xffffffffu, wait_bar(bar, parity, code));
+        tc_fence_after();
+        return r;
+      };
+      auto wait_kv = [&](uint32_t& slot) -> bool {
+        slot = kv_c % NS;
+        const bool r = wait_all(&kv_full[slot], (kv_c / NS) & 1, DEV_TIMEOUT_KV);
+        ++kv_c;
+        return r;
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (leader) tc_commit(bar);
+      };
+      auto issue_s = [&](int h, uint32_t kslot) {
+        const uint64_t qd = smem_desc_sw128(sQa + h * SM::kTile, 16);
+        const uint64_t kd = smem_desc_sw128(sKVa + kslot * SM::kTile, 16);
+        const uint32_t d = tmem + h * 128;
+        if (leader) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint64_t off = ((kk >> 2) * kRegion + (kk & 3) * 32) >> 4;
-            mma_ss(tmem + h * 128, q_desc[h] + off, kd + off, C.idesc_qk, kk > 0);
+            mma_ss(d, qd + off, kd + off, C.idesc_qk, kk > 0);
           }
           tc_commit(&s_full[h]);
-        };
-        // O += P V of half h: the first 64 keys as soon as their P is there
-        auto issue_pv = [&](int h, uint32_t vslot, bool acc) -> bool {
-          const uint32_t d = tmem + 256 + h * D, p = tmem + h * 128 + 64;
-          const uint64_t vd = smem_desc_sw128(sKVa + vslot * SM::kTile, kRegion);
-          if (!wait_bar(&pa_full[h], tp[h] & 1, DEV_TIMEOUT_P)) return false;
-          tc_fence_after();
+        }
+        __syncwarp();
+      };
+      // O += P V of half h: the first 64 keys as soon as their P is there
+      auto issue_pv = [&](int h, uint32_t vslot, bool acc) -> bool {
+        const uint32_t d = tmem + 256 + h * D, p = tmem + h * 128 + 64;
+        const uint64_t vd = smem_desc_sw128(sKVa + vslot * SM::kTile, kRegion);
+        if (!wait_all(&pa_full[h], tp[h] & 1, DEV_TIMEOUT_P)) return false;
+        if (leader) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
             mma_ts(d, p + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), C.idesc_pv,
                    (acc || kk > 0) ? 1u : 0u);
-          if (!wait_bar(&pb_full[h], tp[h] & 1, DEV_TIMEOUT_P)) return false;
-          ++tp[h];
-          tc_fence_after();
+        }
+        __syncwarp();
+        if (!wait_all(&pb_full[h], tp[h] & 1, DEV_TIMEOUT_P)) return false;
+        ++tp[h];
+        if (leader) {
 #pragma unroll
           for (int kk = 4; kk < 8; ++kk)
             mma_ts(d, p + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), C.idesc_pv, 1u);
-          return true;
-        };
-        while (ok) {
-          const uint32_t rs = ring & 1;
-          if (!(ok = wait_bar(&unit_full[rs], (ring >> 1) & 1, DEV_TIMEOUT_ITEM)))
-            break;
-          const int b = s_unit[rs].b, n = s_unit[rs].n, tiles = s_unit[rs].blk1 - s_unit[rs].blk0;
-          mbar_arrive(&unit_empty[rs]);
-          ++ring;
-          if (b < 0) break;
-          if (tiles <= 0) continue;
-          const int halves = n > C.tb ? 2 : 1;
-          for (int h = 0; h < halves && ok; ++h)
-            ok = wait_bar(&q_full[h], tq[h]++ & 1, DEV_TIMEOUT_Q);
-          tc_fence_after();
-          uint32_t ks, vs;
-          if (!ok || !(ok = wait_kv(ks))) break;
-          for (int h = 0; h < halves; ++h) issue_s(h, ks);
-          tc_commit(&kv_empty[ks]);
-          for (int u = 1; u < tiles && ok; ++u) {
-            if (!(ok = wait_kv(vs)) || !(ok = wait_kv(ks))) break;
-            for (int h = 0; h < halves; ++h) {
-              if (!(ok = issue_pv(h, vs, u > 1))) break;
-              issue_s(h, ks);
+        }
+        __syncwarp();
+        return true;
+      };
+      while (ok) {
+        const uint32_t rs = ring & 1;
+        if (!(ok = wait_all(&unit_full[rs], (ring >> 1) & 1, DEV_TIMEOUT_ITEM))) break;
+        auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+        const int b = same(s_unit[rs].b), n = same(s_unit[rs].n);
+        const int blk0 = same(s_unit[rs].blk0), tiles = same(s_unit[rs].blk1) - blk0;
+        const int a0 = same(s_unit[rs].a0), a1 = same(s_unit[rs].a1), n0 = same(s_unit[rs].n0);
+        const int sink_end = same(s_unit[rs].sink_end);
+        HalfTiles ht[2];
+        for (int x = 0; x < 2; ++x) {
+          ht[x].i_hi = same(s_unit[rs].half[x].i_hi);
+          ht[x].live_min = same(s_unit[rs].half[x].live_min);
+        }
+        __syncwarp();
+        if (leader) mbar_arrive(&unit_empty[rs]);
+        ++ring;
+        if (b < 0) break;
+        if (tiles <= 0) continue;
+        const int halves = n > C.tb ? 2 : 1;
+        for (int h = 0; h < halves && ok; ++h) {
+          ok = wait_all(&q_full[h], tq[h] & 1, DEV_TIMEOUT_Q);
+          ++tq[h];
+        }
+        uint32_t ks = 0, vs = 0;
+        bool started[2] = {false, false}, held[2] = {false, false};   // O begun; P V owed
+        // step u: the products with V of super-tile u - 1, then S of super-tile u
+        for (int u = 0; u <= tiles && ok; ++u) {
+          if (u > 0 && !(ok = wait_kv(vs))) break;
+          if (u < tiles && !(ok = wait_kv(ks))) break;
+          const int blk = blk0 + u;
+          const int kb = blk < n0 ? a0 + blk * 128 : a1 + (blk - n0) * 128;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h >= halves) break;
+            if (held[h]) {
+              if (!(ok = issue_pv(h, vs, started[h]))) break;
+              started[h] = true;
             }
-            tc_commit(&kv_empty[vs]);
-            tc_commit(&kv_empty[ks]);
+            held[h] = u < tiles && tile_live(ht[h], kb, sink_end);
+            if (held[h]) issue_s(h, ks);
+            if (u == tiles && started[h]) commit(&o_full[h]);
           }
           if (!ok) break;
-          for (int h = 0; h < halves; ++h) tc_commit(&q_empty[h]);
-          if (!(ok = wait_kv(vs))) break;
-          for (int h = 0; h < halves; ++h) {
-            if (!(ok = issue_pv(h, vs, tiles > 1))) break;
-            tc_commit(&o_full[h]);
-          }
-          tc_commit(&kv_empty[vs]);
+          if (u > 0) commit(&kv_empty[vs]);
+          if (u < tiles) commit(&kv_empty[ks]);
+          if (u == tiles - 1)
+            for (int h = 0; h < halves; ++h) commit(&q_empty[h]);
         }
-        // the commit lands once every product issued above has completed
+      }
+      // the commit lands once every product issued above has completed
+      if (leader) {
         tc_commit(drain);
         const uint64_t t0 = globaltimer();
         while (!mbar_try_wait(drain, 0)) {
           if (globaltimer() - t0 > attn::kDrainLimitNs) { err.record(DEV_TIMEOUT_DRAIN); break; }
         }
       }
+      __syncwarp();
     }
   } else {
     // -------------------------------------------------------------- softmax, results
@@ -418,7 +526,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const uint32_t lane_off = (uint32_t)(wq * 32) << 16;
     const uint32_t tS = tmem + lane_off + h * 128;
     const uint32_t tO = tmem + lane_off + 256 + h * D;
-    uint8_t* stage = smem + SM::kEpiOff + warp * (32 * 128);
     const float c2 = P.scale_log2;
     const int tok = r_in / P.group;                  // token of the half
     const int qh = r_in - tok * P.group;             // query head of the group
@@ -438,51 +545,85 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       const int t_in = h * C.tb + tok;               // token of the unit
       const bool valid = tok < C.tb && t_in < u.n;
       const int i = u.pos0 + t_in;
-      const int i_lo = u.pos0 + h * C.tb, i_hi = u.pos0 + min(u.n, (h + 1) * C.tb) - 1;
-      const int32_t* trow = P.table + (long long)u.b * P.table_stride;
-      const int n0 = (u.runs.cnt[0] + 127) / 128;
-      auto base_of = [&](int blk) {
-        const int part = blk >= n0;
-        return (part ? u.runs.a[1] : u.runs.a[0]) + (blk - (part ? n0 : 0)) * 128;
+      // page of box `lane` of a super-tile, read one ahead and looked at then
+      auto page_of = [&](int blk) -> int {
+        const int4 g = lds4(&u.a0);
+        const int j = (blk < g.z ? g.x + blk * 128 : g.y + (blk - g.z) * 128) + lane * C.seg;
+        return blk < u.blk1 && lane < C.nseg && j < u.len ? __ldg(u.table + (j >> P.page_shift)) : -1;
       };
-      // bit x: box x of the super-tile has keys
-      auto boxes_of = [&](int blk) -> bool {
-        if (blk >= u.blk1 || lane >= C.nseg) return false;
-        const int j = base_of(blk) + lane * C.seg;
-        return j < u.len && (unsigned)__ldg(trow + (j >> P.page_shift)) < (unsigned)P.pages;
-      };
-      bool box = boxes_of(u.blk0);
+      int blk = u.blk0;
+      int page = page_of(blk);
       float m_used = -INFINITY, l = 0.f;
+      bool any = false;                              // a product with V has been asked for
 #pragma unroll 1
-      for (int blk = u.blk0; blk < u.blk1; ++blk) {
-        const uint32_t boxes = __ballot_sync(0xffffffffu, box);
-        box = boxes_of(blk + 1);
-        const int kb = base_of(blk);
-        const bool whole = kb + 128 <= u.len && boxes == (1u << C.nseg) - 1u;
-        const bool full = whole && kb + 127 <= i_lo &&
-                          (P.pred.kind == PA_CAUSAL ||
-                           ((P.pred.kind == PA_WINDOW || P.pred.kind == PA_SINKS) &&
-                            i_hi - kb < P.pred.p0));
+      for (; blk < *const_cast<volatile const int*>(&u.blk1); ++blk) {
+        const int4 g = lds4(&u.a0), ht = lds4(&u.half[h]);
+        const int kb = blk < g.z ? g.x + blk * 128 : g.y + (blk - g.z) * 128;
+        // bit x: box x of the super-tile has keys
+        const uint32_t boxes = __ballot_sync(0xffffffffu, (unsigned)page < (unsigned)P.pages);
+        page = page_of(blk + 1);
+        if (kb > ht.x || (kb < ht.y && kb >= g.w)) continue;
+        const bool all_boxes = boxes == (1u << C.nseg) - 1u;
+        const bool full = kb >= ht.z && kb <= ht.w && all_boxes;
         uint32_t mk[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-        if (!full) {
-          // live bits of this row, box by box (a word of 32 keys at most)
-          const int width = min(C.seg, 32);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t word = 0;
-#pragma unroll 1
-            for (int c0 = k * 32; c0 < k * 32 + 32; c0 += width) {
-              const int sg = c0 / C.seg, in = c0 - sg * C.seg;
-              if (!((boxes >> sg) & 1u)) continue;
-              const int j = kb + sg * C.seg;
-              const int shift = max(C.seg - (u.len - j), 0);   // the last page's end
-              uint32_t bits;
-              if (!progression_bits(P.pred, i - (j - shift), j - shift, 1, 0, in, C.seg, bits))
-                bits = element_bits(P.pred, i, nullptr, j - shift, 1, in, width);
-              bits &= range_bits(shift, C.seg - 1, in);
-              word |= bits << (c0 - k * 32);
+        if (__builtin_expect(!full, 0)) {
+          const int len = u.len;
+          const bool whole = kb + 128 <= len && all_boxes;
+          // Live bits of this row.  The bands are one or two ranges of columns, in closed form;
+          // the columns of the box with the request's last token are shifted, those of
+          // boxes without keys are dead.  The lattices go box by box.
+          const int seg_shift = 31 - __clz(C.seg);
+          const int tail0 = min(((len - kb) >> seg_shift) << seg_shift, 128);   // the shifted box
+          const int shift = tail0 < 128 ? C.seg - (len - kb - tail0) : 0;       // C.seg: it is empty
+          if (P.pred.mod <= 1) {
+            const int c = i - kb;
+            int a0 = 0, b0 = c, a1 = 0, b1 = -1;
+            if (P.pred.kind == PA_WINDOW || P.pred.kind == PA_SINKS || P.pred.kind == PA_TWOBAND)
+              a0 = max(c - P.pred.p0 + 1, 0);
+            if (P.pred.kind == PA_SINKS) b1 = min(P.pred.p1 - 1 - kb, c);
+            if (P.pred.kind == PA_TWOBAND) {
+              a1 = max(c - P.pred.p1 - P.pred.p2 + 1, 0);
+              b1 = min(c - P.pred.p1, c);
             }
-            mk[k] = word;
+            if (P.pred.kind == PA_LOCAL_STRIDED || P.pred.kind == PA_DILATED) a0 = 0;   // every key
+            if (P.pred.kind == PA_FAR_STRIDED) b0 = min(c - P.pred.p0, c);
+            if (whole) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mk[k] = range_bits(a0, b0, k * 32) | range_bits(a1, b1, k * 32);
+            } else {
+              const int last = len - kb - 1;
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mk[k] = range_bits(a0, min(b0, tail0 - 1), k * 32) |
+                        range_bits(a1, min(b1, tail0 - 1), k * 32) |
+                        range_bits(max(a0, tail0) + shift, min(b0, last) + shift, k * 32) |
+                        range_bits(max(a1, tail0) + shift, min(b1, last) + shift, k * 32);
+              for (uint32_t gone = ~boxes & ((1u << C.nseg) - 1u); gone; gone &= gone - 1) {
+                const int c0 = (__ffs(gone) - 1) << seg_shift;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mk[k] &= ~range_bits(c0, c0 + C.seg - 1, k * 32);
+              }
+            }
+          } else {
+            const int width = min(C.seg, 32);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t word = 0;
+#pragma unroll 1
+              for (int c0 = k * 32; c0 < k * 32 + 32; c0 += width) {
+                const int sg = c0 >> seg_shift, in = c0 & (C.seg - 1);
+                if (!((boxes >> sg) & 1u)) continue;
+                const int sh = sg << seg_shift == tail0 ? shift : 0;
+                const int j = kb + (sg << seg_shift) - sh;
+                uint32_t bits;
+                if (!progression_bits(P.pred, i - j, j, 1, 0, in, C.seg, bits))
+                  bits = element_bits(P.pred, i, nullptr, j, 1, in, width);
+                bits &= range_bits(sh, C.seg - 1, in);
+                word |= bits << (c0 - k * 32);
+              }
+              mk[k] = word;
+            }
           }
         }
         ok = wait_bar(&s_full[h], ts & 1, DEV_TIMEOUT_S);
@@ -509,7 +650,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             s[96 + x] = __uint_as_float(r3[x]);
           }
         }
-        if (!full) {
+        if (__builtin_expect(!full, 0)) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -522,31 +663,33 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 #pragma unroll
           for (int j = 0; j < 8; ++j) m8[j] = fmaxf(s[2 * j], s[2 * j + 1]);
 #pragma unroll
-          for (int c = 16; c < 128; c += 16) {
+          for (int c = 16; c < 128; c += 16)
 #pragma unroll
             for (int j = 0; j < 8; ++j) m8[j] = attn::fmax3(m8[j], s[c + 2 * j], s[c + 2 * j + 1]);
-          }
           mx = attn::fmax3(attn::fmax3(m8[0], m8[1], m8[2]), attn::fmax3(m8[3], m8[4], m8[5]),
                            fmaxf(m8[6], m8[7]));
         }
         const float m_tile = mx * c2;
         const bool bump = m_tile > m_used + 8.0f;    // from -inf: the first live key
-        float factor = 1.f;
-        if (bump) {
-          factor = ex2f(m_used - m_tile);
-          m_used = m_tile;
-          l *= factor;
-        }
-        if (__any_sync(0xffffffffu, bump && blk > u.blk0)) {
+        if (__builtin_expect(__any_sync(0xffffffffu, bump), 0)) {
+          float factor = 1.f;
+          if (bump) {
+            factor = ex2f(m_used - m_tile);
+            m_used = m_tile;
+            l *= factor;
+          }
+          if (any) {
 #pragma unroll 1
-          for (int k = 0; k < D / 32; ++k) {
-            uint32_t r[32];
-            tmem_ld32(tO + k * 32, r);
-            tmem_wait_ld();
-            tmem_regs_ready(r);
+            for (int k = 0; k < D / 16; ++k) {
+              uint32_t r[16];
+              tmem_ld16(tO + k * 16, r);
+              tmem_wait_ld();
 #pragma unroll
-            for (int x = 0; x < 32; ++x) r[x] = __float_as_uint(__uint_as_float(r[x]) * factor);
-            tmem_st32(tO + k * 32, r);
+              for (int x = 0; x < 16; ++x) asm volatile("" : "+r"(r[x]));
+#pragma unroll
+              for (int x = 0; x < 16; ++x) r[x] = __float_as_uint(__uint_as_float(r[x]) * factor);
+              tmem_st16(tO + k * 16, r);
+            }
           }
         }
         const float msub = m_used == -INFINITY ? 0.f : m_used;
@@ -559,17 +702,17 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
             const int c = q4 * 32 + 2 * x;
-            float x0, x1, a, b;
+            float x0, x1, e0, e1;
             attn::ffma2(x0, x1, s[c], s[c + 1], c2, -msub);
             if (on_fma<D>(x)) {
-              exp2_poly(x0, x1, a, b);
+              exp2_poly(x0, x1, e0, e1);
             } else {
-              a = ex2f(x0);
-              b = ex2f(x1);
+              e0 = ex2f(x0);
+              e1 = ex2f(x1);
             }
             const int j = (2 * x) & 7;
-            attn::fadd2(r8[j], r8[j + 1], a, b);
-            pk[x] = pack_pair<kBf16>(a, b);
+            attn::fadd2(r8[j], r8[j + 1], e0, e1);
+            pk[x] = pack_pair<kBf16>(e0, e1);
           }
           tmem_st16(tS + 64 + q4 * 16, pk);
           if (q4 & 1) {
@@ -578,12 +721,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             mbar_arrive(q4 == 1 ? &pa_full[h] : &pb_full[h]);
           }
         }
+        any = true;
         l += ((r8[0] + r8[1]) + (r8[2] + r8[3])) + ((r8[4] + r8[5]) + (r8[6] + r8[7]));
       }
       if (!ok) break;
 
       // results: o and lse, or this piece's O, maximum and sum
-      const bool any = u.blk1 > u.blk0;
       const int t = u.row0 + t_in, a = u.h * P.group + qh;
       float* part = u.slot >= 0 ? scratch + (size_t)u.slot * slot_floats<D>(256) : nullptr;
       const int rr = h * 128 + r_in;
@@ -599,70 +742,50 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
       }
+      // every thread writes its row, 32 bytes (a whole sector) at a time where rows are so
+      // aligned
       const float inv_l = part ? 1.f : l > 0.f ? 1.f / l : 0.f;
-      float probe = l - l;
-      const int chunks = part ? D / 32 : D / 64;      // of 128 bytes of a row
+      float probe[4] = {l * 0.f, 0.f, 0.f, 0.f};        // 0 unless something is not finite
 #pragma unroll 1
-      for (int c = 0; c < chunks; ++c) {
-        __syncwarp();                                 // the last chunk has left the stage
-        if (part) {
-          uint32_t r[32];
-          if (any) {
-            tmem_ld32(tO + c * 32, r);
-            tmem_wait_ld();
-            tmem_regs_ready(r);
-          } else {
-#pragma unroll
-            for (int x = 0; x < 32; ++x) r[x] = 0u;
-          }
-#pragma unroll
-          for (int x = 0; x < 32; ++x) probe += __uint_as_float(r[x]) - __uint_as_float(r[x]);
-#pragma unroll
-          for (int x = 0; x < 8; ++x)
-            *reinterpret_cast<uint4*>(stage + lane * 128 + ((x ^ (lane & 7)) << 4)) =
-                make_uint4(r[4 * x], r[4 * x + 1], r[4 * x + 2], r[4 * x + 3]);
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t r[32];
+        if (any) {
+          tmem_ld32(tO + c * 32, r);
+          tmem_wait_ld();
+          tmem_regs_ready(r);
         } else {
-          uint32_t r0[32], r1[32];
-          if (any) {
-            tmem_ld32(tO + c * 64, r0);
-            tmem_ld32(tO + c * 64 + 32, r1);
-            tmem_wait_ld();
-            tmem_regs_ready(r0);
-            tmem_regs_ready(r1);
+#pragma unroll
+          for (int x = 0; x < 32; ++x) r[x] = 0u;
+        }
+#pragma unroll
+        for (int x = 0; x < 32; x += 4) {
+          attn::fma2v(probe[0], probe[1], __uint_as_float(r[x]), __uint_as_float(r[x + 1]), 0.f, 0.f,
+                      probe[0], probe[1]);
+          attn::fma2v(probe[2], probe[3], __uint_as_float(r[x + 2]), __uint_as_float(r[x + 3]), 0.f,
+                      0.f, probe[2], probe[3]);
+        }
+        if (row_ptr) {
+          char* dst = reinterpret_cast<char*>(row_ptr);
+          if (part) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              st32(dst + c * 128 + x * 32, true, r[8 * x], r[8 * x + 1], r[8 * x + 2], r[8 * x + 3],
+                   r[8 * x + 4], r[8 * x + 5], r[8 * x + 6], r[8 * x + 7]);
           } else {
 #pragma unroll
-            for (int x = 0; x < 32; ++x) r0[x] = r1[x] = 0u;
+            for (int x = 0; x < 16; ++x)
+              r[x] = pack_pair<kBf16>(__uint_as_float(r[2 * x]) * inv_l,
+                                      __uint_as_float(r[2 * x + 1]) * inv_l);
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              st32(dst + c * 64 + x * 32, C.o32, r[8 * x], r[8 * x + 1], r[8 * x + 2], r[8 * x + 3],
+                   r[8 * x + 4], r[8 * x + 5], r[8 * x + 6], r[8 * x + 7]);
           }
-#pragma unroll
-          for (int x = 0; x < 32; ++x)
-            probe += (__uint_as_float(r0[x]) - __uint_as_float(r0[x])) +
-                     (__uint_as_float(r1[x]) - __uint_as_float(r1[x]));
-#pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            uint32_t w4[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int col = 8 * (x & 3) + 2 * j;
-              w4[j] = pack_pair<kBf16>(__uint_as_float(x < 4 ? r0[col] : r1[col]) * inv_l,
-                                       __uint_as_float(x < 4 ? r0[col + 1] : r1[col + 1]) * inv_l);
-            }
-            *reinterpret_cast<uint4*>(stage + lane * 128 + ((x ^ (lane & 7)) << 4)) =
-                make_uint4(w4[0], w4[1], w4[2], w4[3]);
-          }
-        }
-        __syncwarp();
-        const int x = lane & 7;
-#pragma unroll
-        for (int it = 0; it < 8; ++it) {
-          const int rw = it * 4 + (lane >> 3);
-          const uint4 v = *reinterpret_cast<const uint4*>(stage + rw * 128 + ((x ^ (rw & 7)) << 4));
-          const unsigned long long dst = __shfl_sync(0xffffffffu, row_ptr, rw);
-          if (dst) *reinterpret_cast<uint4*>(reinterpret_cast<char*>(dst) + c * 128 + x * 16) = v;
         }
       }
       if (any) tc_fence_before();
       // a value that is not finite, seen or weighed by 0: those rows key by key instead
-      uint32_t odd = __ballot_sync(0xffffffffu, valid && probe != 0.f);
+      uint32_t odd = __ballot_sync(0xffffffffu, valid && !((probe[0] + probe[1]) + (probe[2] + probe[3]) == 0.f));
       if (odd) {
         __syncwarp();
         if (lane == 0) atomicAdd(s_slow, 1);          // the other warps' waits hold on
