@@ -6,6 +6,7 @@ raises instead of computing anything on the CPU.
 """
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libpolyattn_sm100.so"
@@ -90,6 +91,16 @@ class PaPagedAttnArgs(ctypes.Structure):
                 ("lse_head_stride", c_i64), ("pred", PaPred), ("scale", c_f32)]
 
 
+def packer(cls):
+    """``struct`` packing of an argument struct, its fields in order (a nested struct's in
+    its place): one call instead of a Python attribute write per field, which is what a
+    small launch spends most of its host time on."""
+    def fmt(c):
+        return "".join(fmt(t) if issubclass(t, ctypes.Structure) else
+                       {c_i32: "i", c_i64: "q", c_vp: "P", c_f32: "f"}[t] for _, t in c._fields_)
+    return struct.Struct("@" + fmt(cls)).pack
+
+
 # name -> (restype, argtypes); every symbol include/polyattn.h declares
 SIGNATURES = {
     "pa_last_error": (ctypes.c_char_p, []),
@@ -110,14 +121,14 @@ SIGNATURES = {
     "pa_attn_fwd_noalloc": (ctypes.c_int, [ctypes.POINTER(PaAttnArgs), c_vp]),
     "pa_attn_noalloc_status": (ctypes.c_int, [ctypes.POINTER(c_i32), c_vp]),
     "pa_lse_merge": (ctypes.c_int, [ctypes.POINTER(PaMergeArgs), c_vp]),
-    "pa_paged_step": (ctypes.c_int, [ctypes.POINTER(PaPagedStepArgs), c_vp]),
-    "pa_paged_plan_size": (c_sz, [ctypes.POINTER(PaPagedAttnArgs)]),
-    "pa_paged_scratch_size": (c_sz, [ctypes.POINTER(PaPagedAttnArgs)]),
-    "pa_paged_plan": (ctypes.c_int, [ctypes.POINTER(PaPagedAttnArgs), c_vp, c_sz, c_vp]),
-    "pa_paged_attn": (ctypes.c_int, [ctypes.POINTER(PaPagedAttnArgs), c_vp, c_sz, c_vp, c_sz,
-                                     c_vp]),
+    # the argument structs of these calls come as bytes (``packer``) or by reference
+    "pa_paged_step": (ctypes.c_int, [c_vp, c_vp]),
+    "pa_paged_plan_size": (c_sz, [c_vp]),
+    "pa_paged_scratch_size": (c_sz, [c_vp]),
+    "pa_paged_plan": (ctypes.c_int, [c_vp, c_vp, c_sz, c_vp]),
+    "pa_paged_attn": (ctypes.c_int, [c_vp, c_vp, c_sz, c_vp, c_sz, c_vp]),
     "pa_paged_status": (ctypes.c_int, [c_vp, ctypes.POINTER(c_i32), c_vp]),
-    "pa_paged_append": (ctypes.c_int, [ctypes.POINTER(PaPagedAppendArgs), c_vp]),
+    "pa_paged_append": (ctypes.c_int, [c_vp, c_vp]),
 }
 
 ABI_VERSION = 8

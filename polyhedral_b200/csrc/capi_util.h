@@ -47,6 +47,31 @@ inline bool aligned(const void* p, size_t a) {
   return (reinterpret_cast<uintptr_t>(p) % a) == 0;
 }
 
+// Launches a kernel that may begin while the kernel before it on the stream still runs
+// (programmatic dependent launch).  Such a kernel calls pdl_wait (common.cuh) in every CTA
+// before it touches memory: it returns when that kernel, and so every earlier one, has
+// completed.
+template <typename... KArgs, typename... Args>
+int launch_after(const char* who, void (*kernel)(KArgs...), int grid, int threads, int smem,
+                 cudaStream_t stream, Args&&... args) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(PA_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
+  }
+  return PA_OK;
+}
+
 namespace attn {
 // Status of the last attention forward on a workspace (device memory), read
 // stream-ordered and synchronising `stream` (csrc/attn.cu).

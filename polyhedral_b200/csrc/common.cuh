@@ -40,6 +40,11 @@ PA_DEV uint64_t globaltimer() {
   return t;
 }
 
+// Kernels launched by launch_after: pdl_wait returns when every kernel before this one on
+// the stream has completed; from pdl_begin_next on, the next one may begin (and wait).
+PA_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+PA_DEV void pdl_begin_next() { asm volatile("griddepcontrol.launch_dependents;"); }
+
 // ----------------------------------------------------------------- mbarrier
 PA_DEV void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));

@@ -2,6 +2,7 @@
 // the keys that a run of query positions can see.
 #pragma once
 #include <math.h>
+#include <atomic>
 #include "common.cuh"
 #include "capi_util.h"
 
@@ -9,6 +10,7 @@ namespace pa {
 namespace paged {
 
 struct Params {
+  uint32_t group_inv;   // (x * group_inv) >> 20 = x / group for 0 <= x < 512
   const void* q;
   const void* k;
   const void* v;
@@ -25,6 +27,12 @@ struct Params {
   float scale_log2;
 };
 
+// x / group for 0 <= x < 512: group_inv = ceil(2^20 / group) is above 2^20 / group by less
+// than 1, which shifts the product by less than 512 / 2^20 < 1 / (8 * 128).
+__device__ __forceinline__ int div_group(const Params& P, int x) {
+  return (int)(((uint32_t)x * P.group_inv) >> 20);
+}
+
 // A request as the kernels see it: its first row of q / o, its new tokens, the position of the
 // first of them, and its tokens, all kept inside the buffers whatever the arrays say.
 struct Request {
@@ -38,7 +46,9 @@ __device__ __forceinline__ Request get_request(const Params& P, int b) {
   const int len = __ldg(P.seq_lens + b);
   // a token's position counts back from the request's last one, also where the table
   // is too narrow for all of them
-  r.pos0 = len - (e - s) + (r.row0 - s);
+  // (kept within 2^26, so that no sum with a mask's widths overflows)
+  const long long pos = (long long)len - ((long long)e - s) + ((long long)r.row0 - s);
+  r.pos0 = (int)max(min(pos, 1ll << 26), -(1ll << 26));
   r.len = min(max(len, 0), P.width << P.page_shift);
   return r;
 }
@@ -50,30 +60,29 @@ struct KeyRanges {
   int a0, b0, a1, b1;
 };
 __device__ __forceinline__ KeyRanges key_ranges(const Pred& p, int i0, int i1, int len) {
-  typedef long long ll;
-  ll hi = min((ll)i1 + 1, (ll)len);
-  ll a = 0, b = hi, c = 0, d = 0;   // near [a, b), far [c, d)
+  const int hi = min(i1 + 1, len);
+  int a = 0, b = hi, c = 0, d = 0;   // near [a, b), far [c, d)
   switch (p.kind) {
     case PA_WINDOW:
-      a = (ll)i0 - p.p0 + 1;
+      a = i0 - p.p0 + 1;
       break;
     case PA_SINKS:
-      a = (ll)i0 - p.p0 + 1;
+      a = i0 - p.p0 + 1;
       d = p.p1;
       break;
     case PA_TWOBAND:
-      a = (ll)i0 - p.p0 + 1;
-      c = (ll)i0 - p.p1 - p.p2 + 1;
-      d = (ll)i1 - p.p1 + 1;
+      a = i0 - p.p0 + 1;
+      c = i0 - p.p1 - p.p2 + 1;
+      d = i1 - p.p1 + 1;
       break;
     case PA_FAR_STRIDED:
-      b = (ll)i1 - p.p0 + 1;
+      b = i1 - p.p0 + 1;
       break;
     default:
       break;
   }
-  a = max(a, 0ll);
-  c = max(c, 0ll);
+  a = max(a, 0);
+  c = max(c, 0);
   b = min(b, hi);
   d = min(d, hi);
   KeyRanges r{0, 0, 0, 0};
@@ -81,7 +90,7 @@ __device__ __forceinline__ KeyRanges key_ranges(const Pred& p, int i0, int i1, i
   if (c >= d) c = d = 0;
   if (a < b && c < d) {
     if (c > a) {
-      ll t = a; a = c; c = t;
+      int t = a; a = c; c = t;
       t = b; b = d; d = t;
     }
     if (d >= a) {       // they touch: one range
@@ -91,15 +100,38 @@ __device__ __forceinline__ KeyRanges key_ranges(const Pred& p, int i0, int i1, i
     }
   }
   if (c < d) {
-    r.a0 = (int)c;
-    r.b0 = (int)d;
-    r.a1 = (int)a;
-    r.b1 = (int)b;
+    r.a0 = c;
+    r.b0 = d;
+    r.a1 = a;
+    r.b1 = b;
   } else {
-    r.a0 = (int)a;
-    r.b0 = (int)b;
+    r.a0 = a;
+    r.b0 = b;
   }
   return r;
+}
+
+// Allows kernel kKernel `smem` bytes of shared memory, once per device; with `min_regs`,
+// refuses a build with fewer registers per thread (a register split that they do not cover
+// would never complete).
+template <auto kKernel>
+int prepare_kernel(int smem, int min_regs) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  PA_CUDA(cudaGetDevice(&dev), "pa_paged_attn");
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return PA_OK;
+  PA_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+          "pa_paged_attn");
+  if (min_regs > 0) {
+    cudaFuncAttributes fa;
+    PA_CUDA(cudaFuncGetAttributes(&fa, kKernel), "pa_paged_attn");
+    if (fa.numRegs < min_regs)
+      return fail(PA_ERR_UNSUPPORTED, "pa_paged_attn: kernel built with %d registers per thread, "
+                  "below its register split", fa.numRegs);
+  }
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return PA_OK;
 }
 
 // ------------------------------------------------------------- shares of work
@@ -110,8 +142,14 @@ __device__ __forceinline__ KeyRanges key_ranges(const Pred& p, int i0, int i1, i
 // workers, whose partial results (sum, running maximum and unnormalised O of every row,
 // 32-bit) are joined by a second kernel in the order of the keys.  No counters, no order
 // that depends on timing: the same call gives the same bits.
-struct Share {
+struct __align__(16) Share {
   int b, h, t, blk;   // request, key head, unit of them, first block
+  Request R;          // the request, so that a worker starts without a chain of loads
+};
+// A divided unit: the worker that begins it, its pieces, and where its rows are.
+struct __align__(16) Cut {
+  int worker, pieces, h, t;
+  Request R;
 };
 
 // What the host chooses from the sizes and hints alone, alike for plan and forward.
@@ -130,12 +168,11 @@ struct PlanView {
   int32_t* status;
   int32_t* meta;      // shares in use, divided units, most rows of a unit
   Share* shares;      // [workers + 1]
-  int32_t* cuts;      // [workers] workers that begin a divided unit
+  Cut* cuts;          // [workers] divided units
   long long* before;  // [requests + 1] cost before a request
 };
 inline __host__ size_t plan_bytes(const Config& c, int requests) {
-  return 256 + sizeof(Share) * (c.workers + 1) + 4 * (size_t)((c.workers + 1) & ~1) +
-         8 * (size_t)(requests + 1);
+  return 256 + sizeof(Share) * (c.workers + 1) + sizeof(Cut) * c.workers + 8 * (size_t)(requests + 1);
 }
 inline __host__ PlanView plan_view(void* p, const Config& c) {
   char* b = static_cast<char*>(p);
@@ -143,9 +180,8 @@ inline __host__ PlanView plan_view(void* p, const Config& c) {
   v.status = reinterpret_cast<int32_t*>(b);
   v.meta = reinterpret_cast<int32_t*>(b + 64);
   v.shares = reinterpret_cast<Share*>(b + 256);
-  v.cuts = reinterpret_cast<int32_t*>(b + 256 + sizeof(Share) * (c.workers + 1));
-  v.before = reinterpret_cast<long long*>(b + 256 + sizeof(Share) * (c.workers + 1) +
-                                          4 * (size_t)((c.workers + 1) & ~1));
+  v.cuts = reinterpret_cast<Cut*>(b + 256 + sizeof(Share) * (c.workers + 1));
+  v.before = reinterpret_cast<long long*>(v.cuts + c.workers);
   return v;
 }
 
@@ -175,12 +211,11 @@ __device__ __forceinline__ Runs unit_runs(const Pred& p, int i0, int i1, int len
     const int top = min(i0, len - 1);
     const int near = p.kind == PA_LOCAL_STRIDED ? min(max(p.p0, 0), i0 + 1) : 0;   // band's keys
     const int far0 = p.kind == PA_FAR_STRIDED ? max(p.p0, 0) : near;
-    const long long last = min((long long)top, (long long)i0 - far0);
+    const int last = min(top, i0 - far0);
     const int first = i0 >= 0 ? i0 % p.mod : 0;
-    // the last lattice key at or below `last`
     r.a[0] = r.lo[0] = first;
     r.step[0] = p.mod;
-    r.cnt[0] = i0 >= 0 && last >= first ? (int)((last - first) / p.mod) + 1 : 0;
+    r.cnt[0] = i0 >= 0 && last >= first ? (last - first) / p.mod + 1 : 0;
     r.lo[1] = max(i0 - near + 1, 0);
     r.a[1] = r.lo[1] & ~(kBlock - 1);
     r.cnt[1] = near > 0 ? max(top + 1 - r.a[1], 0) : 0;

@@ -214,7 +214,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       }
     }
   };
-  asm volatile("griddepcontrol.launch_dependents;");
+  pdl_wait();
+  pdl_begin_next();
   if ((int)blockIdx.x >= __ldg(meta)) return;   // no share: the whole CTA leaves
 
   if (threadIdx.x == 0) {
@@ -275,7 +276,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           if (at.b >= P.requests || at.b > end.b ||
               (at.b == end.b && (at.h > end.h || (at.h == end.h && at.t > end.t))))
             break;
-          const Request R = get_request(P, at.b);
+          Request R = first.R;
+          if (fresh && at.b == first.b) R.len = min(R.len, P.width << P.page_shift);
+          else R = get_request(P, at.b);
           if (at.t * per >= R.n) {
             at.t = 0;
             if (R.n == 0 || ++at.h == P.kv_heads) {
@@ -843,28 +846,15 @@ int launch_chunk_d64(const CUtensorMap& tq, const CUtensorMap& tk, const CUtenso
                      const ChunkParams& C, bool bf16, const PlanView& pv, float* scratch, int sms,
                      cudaStream_t stream);
 
-template <int D>
+template <int D, bool kBf16>
 int launch_chunk_body(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                      const ChunkParams& C, bool bf16, const PlanView& pv, float* scratch, int sms,
+                      const ChunkParams& C, const PlanView& pv, float* scratch, int sms,
                       cudaStream_t stream) {
-  auto go = [&](auto kernel) -> int {
-    PA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 ChunkSmem<D>::kAlloc), "pa_paged_attn");
-    // the warpgroups' register shares must fit in the registers of the launch
-    static std::atomic<int> regs_ok{0};
-    cudaFuncAttributes fa;
-    fa.numRegs = 1 << 20;
-    if (!regs_ok.load(std::memory_order_relaxed))
-      PA_CUDA(cudaFuncGetAttributes(&fa, kernel), "pa_paged_attn");
-    if (fa.numRegs * kChunkThreads < 256 * kChunkSoftRegs + 128 * kChunkOtherRegs)
-      return fail(PA_ERR_UNSUPPORTED, "pa_paged_attn: kernel built with %d registers per thread, "
-                  "below its register split", fa.numRegs);
-    regs_ok.store(1, std::memory_order_relaxed);
-    kernel<<<sms, kChunkThreads, ChunkSmem<D>::kAlloc, stream>>>(tq, tk, tv, C, pv.shares, pv.meta,
-                                                                 scratch);
-    return check_launch("pa_paged_attn");
-  };
-  return bf16 ? go(paged_chunk_kernel<D, true>) : go(paged_chunk_kernel<D, false>);
+  constexpr int kMinRegs = (256 * kChunkSoftRegs + 128 * kChunkOtherRegs) / kChunkThreads;
+  const int rc = prepare_kernel<paged_chunk_kernel<D, kBf16>>(ChunkSmem<D>::kAlloc, kMinRegs);
+  if (rc) return rc;
+  return launch_after("pa_paged_attn", paged_chunk_kernel<D, kBf16>, sms, kChunkThreads,
+                      ChunkSmem<D>::kAlloc, stream, tq, tk, tv, C, pv.shares, pv.meta, scratch);
 }
 
 }  // namespace paged

@@ -6,7 +6,8 @@ namespace paged {
 int launch_chunk_d64(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                     const ChunkParams& C, bool bf16, const PlanView& pv, float* scratch, int sms,
                     cudaStream_t stream) {
-  return launch_chunk_body<64>(tq, tk, tv, C, bf16, pv, scratch, sms, stream);
+  return bf16 ? launch_chunk_body<64, true>(tq, tk, tv, C, pv, scratch, sms, stream)
+              : launch_chunk_body<64, false>(tq, tk, tv, C, pv, scratch, sms, stream);
 }
 }  // namespace paged
 }  // namespace pa

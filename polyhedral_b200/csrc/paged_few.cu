@@ -9,7 +9,6 @@
 // the warp's matrix instructions (16 rows x 16 keys): idle rows cost nothing that
 // is short here, and the 5th-generation tensor path would bring tensor memory and
 // CTA-wide barriers to a kernel that spends a tenth of its issue slots.
-#include <atomic>
 #include "paged.cuh"
 
 namespace pa {
@@ -37,12 +36,12 @@ template <bool kBf16>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
   if constexpr (kBf16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3},"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3},"
                  " {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3},"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3},"
                  " {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -103,14 +102,16 @@ paged_few_kernel(const __grid_constant__ Params P, const Share* __restrict__ sha
   using F = Few<D>;
   constexpr int S = F::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
-  asm volatile("griddepcontrol.launch_dependents;");
+  pdl_wait();
+  pdl_begin_next();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // neighbouring shares go to different multiprocessors, so that little work spreads
   const int w = warp * gridDim.x + blockIdx.x;
-  if (w >= __ldg(meta)) return;
   const uint32_t ring = smem_u32(smem) + warp * F::kWarpBytes;
   uint32_t* s_live = reinterpret_cast<uint32_t*>(smem + F::kMetaOff) + warp * S;
-  const Share first = shares[w], end = shares[w + 1];
+  const int used = __ldg(meta);
+  const Share first = shares[w], end = shares[w + 1];   // inside the plan for every worker
+  if (w >= used) return;
   const int G = P.group;
   const int mask = (1 << P.page_shift) - 1;
   const int g = lane >> 2, tq = lane & 3;      // fragment row and column pair of this lane
@@ -123,7 +124,12 @@ paged_few_kernel(const __grid_constant__ Params P, const Share* __restrict__ sha
         (at.b == end.b && (at.h > end.h || (at.h == end.h && at.t > end.t))))
       break;
     Piece c;
-    c.R = get_request(P, at.b);
+    if (fresh && at.b == first.b) {
+      c.R = first.R;
+      c.R.len = min(c.R.len, P.width << P.page_shift);
+    } else {
+      c.R = get_request(P, at.b);
+    }
     const int total = c.R.n * G;
     if (at.t * kFewRows >= total) {            // past the request's last unit
       at.t = 0;
@@ -139,7 +145,9 @@ paged_few_kernel(const __grid_constant__ Params P, const Share* __restrict__ sha
     c.h = at.h;
     c.row0 = at.t * kFewRows;
     c.rows = min(total - c.row0, kFewRows);
-    const int i0 = c.R.pos0 + c.row0 / G, i1 = c.R.pos0 + (c.row0 + c.rows - 1) / G;
+    const int t0 = c.row0 / G, in0 = c.row0 - t0 * G;      // first token, head inside it
+    auto token = [&](int r) { return t0 + div_group(P, in0 + r); };
+    const int i0 = c.R.pos0 + t0, i1 = c.R.pos0 + token(c.rows - 1);
     c.runs = unit_runs<kFewBlock, false>(P.pred, i0, i1, c.R.len);
     const int nblk = run_blocks<kFewBlock>(c.runs);
     c.blk0 = fresh ? min(first.blk, nblk) : 0;
@@ -154,59 +162,73 @@ paged_few_kernel(const __grid_constant__ Params P, const Share* __restrict__ sha
     uint32_t qa[D / 16][4];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const int r = g + half * 8;
-      const int row = c.row0 + min(r, c.rows - 1);
-      const uint16_t* qp = static_cast<const uint16_t*>(P.q) +
-                           (long long)(c.R.row0 + row / G) * P.q_t +
-                           (long long)(c.h * G + row % G) * P.q_h + tq * 2;
+      const int r = min(g + half * 8, c.rows - 1), t = token(r);
+      const uint16_t* qp = static_cast<const uint16_t*>(P.q) + (long long)(c.R.row0 + t) * P.q_t +
+                           (long long)(c.h * G + c.row0 + r - t * G) * P.q_h + tq * 2;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         qa[kk][half] = *reinterpret_cast<const uint32_t*>(qp + kk * 16);
         qa[kk][half + 2] = *reinterpret_cast<const uint32_t*>(qp + kk * 16 + 8);
       }
     }
-    const int ig = c.R.pos0 + (c.row0 + min(g, c.rows - 1)) / G;
-    const int ig8 = c.R.pos0 + (c.row0 + min(g + 8, c.rows - 1)) / G;
+    const int ig = c.R.pos0 + token(min(g, c.rows - 1));
+    const int ig8 = c.R.pos0 + token(min(g + 8, c.rows - 1));
 
     const uint16_t* kh = static_cast<const uint16_t*>(P.k) + (long long)c.h * P.k_h;
     const uint16_t* vh = static_cast<const uint16_t*>(P.v) + (long long)c.h * P.v_h;
     const int32_t* trow = P.table + (long long)c.b * P.table_stride;
 
-    // page of place (lane & 15) of block blk, read a block ahead of its rows
+    // Page of block blk, read a block ahead of its rows: a block of consecutive keys starts
+    // at a multiple of 16 and lies in one page; of a lattice every lane reads its own key's.
     auto page_of = [&](int blk) -> int {
       if (blk >= c.blk1) return -1;
       const BlockKeys k = block_keys<kFewBlock>(c.runs, blk);
+      if (k.step == 1) return __ldg(trow + (k.j0 >> P.page_shift));
       const int x = lane & 15;
-      if (x < k.lo || x >= k.hi) return -1;
-      return __ldg(trow + ((k.j0 + x * k.step) >> P.page_shift));
+      return x < k.hi ? __ldg(trow + ((k.j0 + x * k.step) >> P.page_shift)) : -1;
     };
     // issue the copies of block blk into its stage; rows that are not listed become 0
+    constexpr int kChunks = D / 8;                 // 16-byte chunks of a row
+    constexpr int kPer = 32 / kChunks;             // rows per warp-wide copy
+    const int cx = lane % kChunks, rx = lane / kChunks;
     auto load = [&](int blk, int page) {
       if (blk < c.blk1) {
         const int st = (blk - c.blk0) % S;
         const BlockKeys k = block_keys<kFewBlock>(c.runs, blk);
-        const int j = k.j0 + (lane & 15) * k.step;
+        const uint32_t dk = ring + st * 2 * F::kTile + rx * F::kRowBytes, dv = dk + F::kTile;
         const bool ok = (unsigned)page < (unsigned)P.pages;
-        const uint32_t live = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-        long long ko = 0, vo = 0;
-        if (ok) {
-          ko = page * P.k_p + (j & mask) * P.k_r;
-          vo = page * P.v_p + (j & mask) * P.v_r;
-        }
-        const uint32_t dk = ring + st * 2 * F::kTile, dv = dk + F::kTile;
-        if (lane == 0) s_live[st] = live;
-        constexpr int kChunks = D / 8;                 // 16-byte chunks of a row
-        constexpr int kPer = 32 / kChunks;             // rows per warp-wide copy
-        const int cx = lane % kChunks;
+        uint32_t live;
+        if (k.step == 1) {
+          live = ok ? ((1u << k.hi) - 1u) & ~((1u << k.lo) - 1u) : 0u;
+          const int row = (k.j0 & mask) + rx;
+          const uint16_t* kp = kh + (ok ? page * P.k_p + row * P.k_r : 0) + cx * 8;
+          const uint16_t* vp = vh + (ok ? page * P.v_p + row * P.v_r : 0) + cx * 8;
 #pragma unroll
-        for (int i = 0; i < kFewBlock / kPer; ++i) {
-          const int r = i * kPer + lane / kChunks;
-          const long long a = __shfl_sync(0xffffffffu, ko, r), b = __shfl_sync(0xffffffffu, vo, r);
-          const int bytes = (live >> r) & 1 ? 16 : 0;
-          const uint32_t d = r * F::kRowBytes + ((cx ^ (r & 7)) << 4);
-          cp16(dk + d, kh + a + cx * 8, bytes);
-          cp16(dv + d, vh + b + cx * 8, bytes);
+          for (int i = 0; i < kFewBlock / kPer; ++i) {
+            const int r = i * kPer + rx;
+            const int bytes = (live >> r) & 1 ? 16 : 0;
+            const uint32_t d = i * kPer * F::kRowBytes + ((cx ^ (r & 7)) << 4);
+            cp16(dk + d, kp, bytes);
+            cp16(dv + d, vp, bytes);
+            kp += kPer * P.k_r;
+            vp += kPer * P.v_r;
+          }
+        } else {
+          live = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+          const int j = k.j0 + (lane & 15) * k.step;
+          const long long ko = ok ? page * P.k_p + (j & mask) * P.k_r : 0;
+          const long long vo = ok ? page * P.v_p + (j & mask) * P.v_r : 0;
+#pragma unroll 2
+          for (int i = 0; i < kFewBlock / kPer; ++i) {
+            const int r = i * kPer + rx;
+            const long long a = __shfl_sync(0xffffffffu, ko, r), b = __shfl_sync(0xffffffffu, vo, r);
+            const int bytes = (live >> r) & 1 ? 16 : 0;
+            const uint32_t d = i * kPer * F::kRowBytes + ((cx ^ (r & 7)) << 4);
+            cp16(dk + d, kh + a + cx * 8, bytes);
+            cp16(dv + d, vh + b + cx * 8, bytes);
+          }
         }
+        if (lane == 0) s_live[st] = live;
       }
       cp_commit();
     };
@@ -228,25 +250,36 @@ paged_few_kernel(const __grid_constant__ Params P, const Share* __restrict__ sha
       const int next = page_of(blk + S);
       cp_wait<S - 2>();
       __syncwarp();
-      load(blk + S - 1, page);        // into the stage that the last round has read
-      page = next;
       const int st = (blk - c.blk0) % S;
       const uint32_t sk = ring + st * 2 * F::kTile, sv = sk + F::kTile;
       const uint32_t live = s_live[st];
       const BlockKeys k = block_keys<kFewBlock>(c.runs, blk);
 
+      // two sums of D / 2 products each, so that half as many wait for one another
       float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+      float u0[4] = {0.f, 0.f, 0.f, 0.f}, u1[4] = {0.f, 0.f, 0.f, 0.f};
       {
         // matrices: keys 0-7 and 8-15 by the two 16-byte halves of 16 columns
         const int r = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
         const uint32_t base = sk + r * F::kRowBytes;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          uint32_t b[4];
+        for (int kk = 0; kk < D / 16; kk += 2) {
+          uint32_t b[4], b2[4];
           ldm4(base + (((kk * 2 + half) ^ (r & 7)) << 4), b);
+          ldm4(base + (((kk * 2 + 2 + half) ^ (r & 7)) << 4), b2);
           mma16816<kBf16>(s0, qa[kk], b[0], b[1]);
           mma16816<kBf16>(s1, qa[kk], b[2], b[3]);
+          mma16816<kBf16>(u0, qa[kk + 1], b2[0], b2[1]);
+          mma16816<kBf16>(u1, qa[kk + 1], b2[2], b2[3]);
         }
+      }
+      // the next copies go into the stage that the last round has read, while the products run
+      load(blk + S - 1, page);
+      page = next;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s0[e] += u0[e];
+        s1[e] += u1[e];
       }
       // this lane's keys: places 2 tq, 2 tq + 1, 8 + 2 tq, 9 + 2 tq; rows g (0, 1) and g + 8 (2, 3)
       float x[2][4] = {{s0[0], s0[1], s1[0], s1[1]}, {s0[2], s0[3], s1[2], s1[3]}};
@@ -340,7 +373,7 @@ paged_few_kernel(const __grid_constant__ Params P, const Share* __restrict__ sha
           if (tq == 0)
             *reinterpret_cast<float2*>(c.slot + kFewRows * D + 2 * r) = make_float2(m, l);
         } else {
-          const int row = c.row0 + r, t = c.R.row0 + row / G, a = c.h * G + row % G;
+          const int tk = token(r), t = c.R.row0 + tk, a = c.h * G + c.row0 + r - tk * G;
           const float inv = l > 0.f ? 1.f / l : 0.f;
           uint16_t* o = static_cast<uint16_t*>(P.o) + (long long)t * P.o_t + (long long)a * P.o_h + tq * 2;
 #pragma unroll
@@ -359,19 +392,24 @@ paged_few_kernel(const __grid_constant__ Params P, const Share* __restrict__ sha
 
 }  // namespace
 
+namespace {
+template <int D, bool kBf16>
+int launch_few_body(const Params& P, const PlanView& pv, float* scratch, int sms,
+                    cudaStream_t stream) {
+  const int rc = prepare_kernel<paged_few_kernel<D, kBf16>>(Few<D>::kBytes, 0);
+  if (rc) return rc;
+  return launch_after("pa_paged_attn", paged_few_kernel<D, kBf16>, sms, kFewWarps * 32, Few<D>::kBytes,
+                      stream, P, pv.shares, pv.meta, scratch);
+}
+}  // namespace
+
 int launch_few(const Params& P, bool bf16, int D, const PlanView& pv, const Config& c,
                float* scratch, int sms, cudaStream_t stream) {
-  auto go = [&](auto kernel, int smem) -> int {
-    PA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-            "pa_paged_attn");
-    kernel<<<sms, kFewWarps * 32, smem, stream>>>(P, pv.shares, pv.meta, scratch);
-    return check_launch("pa_paged_attn");
-  };
   if (D == 128)
-    return bf16 ? go(paged_few_kernel<128, true>, Few<128>::kBytes)
-                : go(paged_few_kernel<128, false>, Few<128>::kBytes);
-  return bf16 ? go(paged_few_kernel<64, true>, Few<64>::kBytes)
-              : go(paged_few_kernel<64, false>, Few<64>::kBytes);
+    return bf16 ? launch_few_body<128, true>(P, pv, scratch, sms, stream)
+                : launch_few_body<128, false>(P, pv, scratch, sms, stream);
+  return bf16 ? launch_few_body<64, true>(P, pv, scratch, sms, stream)
+              : launch_few_body<64, false>(P, pv, scratch, sms, stream);
 }
 
 }  // namespace paged

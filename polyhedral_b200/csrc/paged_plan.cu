@@ -35,9 +35,14 @@ __device__ __forceinline__ int unit_rows_used(const Params& P, const Config& c, 
 __global__ void __launch_bounds__(kPlanThreads)
 paged_plan_kernel(const __grid_constant__ Params P, Config c, PlanView pv) {
   __shared__ long long warp_sum[kPlanThreads / 32];
+  __shared__ long long s_before[kPlanThreads + 1];   // `before`, where it fits
+  __shared__ int4 s_shares[kPlanThreads + 1];        // b, h, t, blk of a round's shares
   __shared__ int s_rows, s_cuts;
+  pdl_wait();
+  pdl_begin_next();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int B = P.requests;
+  long long* pre = B <= kPlanThreads ? s_before : pv.before;
   if (threadIdx.x == 0) {
     s_rows = s_cuts = 0;
     *pv.status = 0;
@@ -85,23 +90,37 @@ paged_plan_kernel(const __grid_constant__ Params P, Config c, PlanView pv) {
       if (i < warp) before += s;
       all += s;
     }
-    if (b < B) pv.before[b] = before + x - cost;
+    if (b < B) pre[b] = before + x - cost;
     base += all;
     __syncthreads();
   }
-  if (threadIdx.x == 0) pv.before[B] = base;
+  if (threadIdx.x == 0) pre[B] = base;
 #pragma unroll
   for (int o = 16; o; o >>= 1) rows = max(rows, __shfl_xor_sync(0xffffffffu, rows, o));
   if (lane == 0) atomicMax(&s_rows, rows);
   __syncthreads();
   const long long total = base;
-  long long share = (total + c.workers - 1) / c.workers;
-  if (share < c.min_share) share = c.min_share;
-  const int used = total > 0 ? (int)((total + share - 1) / share) : 0;
+  long long share;
+  int used;
+  if (total <= 0x7fff0000ll) {
+    const uint32_t t32 = (uint32_t)total;
+    const uint32_t s32 = max((t32 + c.workers - 1) / c.workers, (uint32_t)c.min_share);
+    share = s32;
+    used = (int)((t32 + s32 - 1) / s32);
+  } else {
+    share = (total + c.workers - 1) / c.workers;
+    used = (int)((total + share - 1) / share);
+  }
 
-  for (int w0 = warp * 32; w0 <= used; w0 += kPlanThreads) {
-    const int w = w0 + lane;
-    Share sh{B, 0, 0, 0};
+  // Rounds of shares, of which each knows the next round's first too.  Divided units are
+  // entered by the worker of their last piece: the worker that begins one is the nearest
+  // earlier one whose share ends inside a unit that it has begun (a running maximum).
+  __shared__ int warp_max[kPlanThreads / 32];
+  int carry = -1;
+  constexpr int kRound = kPlanThreads - 1;
+  for (int wb = 0; wb < used; wb += kRound) {
+    const int w = wb + threadIdx.x;
+    Share sh{B, 0, 0, 0, {0, 0, 0, 0}};
     long long rem = 0;
     Request R{0, 0, 0, 0};
     int n = 0;
@@ -111,12 +130,19 @@ paged_plan_kernel(const __grid_constant__ Params P, Config c, PlanView pv) {
       int lo = 0, hi = B;
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (pv.before[mid] <= x) lo = mid; else hi = mid;
+        if (pre[mid] <= x) lo = mid; else hi = mid;
       }
       sh.b = lo;
-      const long long per_head = (pv.before[lo + 1] - pv.before[lo]) / P.kv_heads;
-      sh.h = (int)((x - pv.before[lo]) / per_head);
-      rem = x - pv.before[lo] - sh.h * per_head;
+      const long long all = pre[lo + 1] - pre[lo], in_b = x - pre[lo];
+      if (all <= 0x7fffffffll) {                      // the usual case, in 32 bits
+        const uint32_t per_head = (uint32_t)all / (uint32_t)P.kv_heads;
+        sh.h = (int)((uint32_t)in_b / per_head);
+        rem = (uint32_t)in_b - sh.h * per_head;
+      } else {
+        const long long per_head = all / P.kv_heads;
+        sh.h = (int)(in_b / per_head);
+        rem = in_b - sh.h * per_head;
+      }
       R = get_request(P, lo);
       n = unit_count(P, c, R);
       if (n <= 4) {
@@ -170,19 +196,40 @@ paged_plan_kernel(const __grid_constant__ Params P, Config c, PlanView pv) {
           sh.t = 0;
           if (++sh.h == P.kv_heads) {
             sh.h = 0;
-            ++sh.b;
+            R = ++sh.b < B ? get_request(P, sh.b) : Request{0, 0, 0, 0};
           }
         }
       }
+      sh.R = R;
     }
     if (w <= used) pv.shares[w] = sh;
-  }
-  __syncthreads();
-  // the workers that begin a unit which a later one goes on with
-  for (int w = threadIdx.x; w < used; w += kPlanThreads) {
-    const Share s = pv.shares[w], e = pv.shares[w + 1];
+    s_shares[threadIdx.x] = make_int4(sh.b, sh.h, sh.t, sh.blk);
+    __syncthreads();
+    const Share& s = sh;
+    const bool mine = w < used && (int)threadIdx.x < kRound;
+    const int4 en = s_shares[mine ? threadIdx.x + 1 : threadIdx.x];
+    const Share e{en.x, en.y, en.z, en.w, {0, 0, 0, 0}};
     const bool same = s.b == e.b && s.h == e.h && s.t == e.t;
-    if (e.blk > 0 && (!same || s.blk == 0)) pv.cuts[atomicAdd(&s_cuts, 1)] = w;
+    const bool begins = mine && e.blk > 0 && (!same || s.blk == 0);
+    int x = begins ? w : -1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x = max(x, y);
+    }
+    __syncthreads();
+    if (lane == 31) warp_max[warp] = x;
+    __syncthreads();
+    int before = carry;
+    for (int i = 0; i < warp; ++i) before = max(before, warp_max[i]);
+    int all = carry;
+    for (int i = 0; i < kPlanThreads / 32; ++i) all = max(all, warp_max[i]);
+    // the running maximum before this worker
+    int w0 = __shfl_up_sync(0xffffffffu, x, 1);
+    w0 = max(lane == 0 ? -1 : w0, before);
+    carry = all;
+    if (mine && s.blk > 0 && !same)
+      pv.cuts[atomicAdd(&s_cuts, 1)] = Cut{w0, w - w0 + 1, s.h, s.t, s.R};
   }
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -206,7 +253,8 @@ paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
   __shared__ float s_acc[kJoinWarps][D];
   __shared__ float2 s_ml[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  pdl_wait();
+  pdl_begin_next();
   const int used = pv.meta[0], cuts = pv.meta[1], rows = pv.meta[2];
   const bool many = used > kJoinWarps * cuts;   // pieces per unit, on average
   const int items = cuts * rows;
@@ -215,9 +263,9 @@ paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
   const int first = many ? blockIdx.x : blockIdx.x * kJoinWarps + warp;
   const int step = many ? gridDim.x : gridDim.x * kJoinWarps;
   for (int it = first; it < items; it += step) {
-    const int w0 = pv.cuts[it / rows], r = it % rows;
-    const Share e0 = pv.shares[w0 + 1];          // the unit
-    const Request R = get_request(P, e0.b);
+    const Cut cut = pv.cuts[it / rows];
+    const int w0 = cut.worker, pieces = cut.pieces, r = it % rows;
+    const Request R = cut.R;
     int tok, g;                                  // token of the request, head of the group
     bool there;
     if (c.half_tokens) {
@@ -225,23 +273,15 @@ paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
       tok = x / P.group;
       g = x - tok * P.group;
       there = tok < c.half_tokens;
-      tok += (e0.t * 2 + (r >> 7)) * c.half_tokens;
+      tok += (cut.t * 2 + (r >> 7)) * c.half_tokens;
       there = there && tok < R.n;
     } else {
-      const int row = e0.t * kFewRows + r;
+      const int row = cut.t * kFewRows + r;
       tok = row / P.group;
       g = row - tok * P.group;
       there = tok < R.n;
     }
     if (!there) continue;                        // alike for the whole CTA, where it shares a row
-    // the last worker on this unit
-    int w1 = w0 + 1;
-    while (w1 + 1 <= used) {
-      const Share e = pv.shares[w1 + 1];
-      if (!(e.b == e0.b && e.h == e0.h && e.t == e0.t)) break;
-      ++w1;
-    }
-    const int pieces = w1 - w0 + 1;
     float m = -INFINITY, l = 0.f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
@@ -308,7 +348,7 @@ paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
         for (int e = 0; e < E; ++e) acc[e] = fmaf(g, s_acc[i][lane * E + e], acc[e]);
       }
     }
-    const int t = R.row0 + tok, a = e0.h * P.group + g;
+    const int t = R.row0 + tok, a = cut.h * P.group + g;
     const float inv = l == 0.f ? 0.f : 1.f / l;   // a sum that is no number stays one
     uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(P.o) + (long long)t * P.o_t +
                                               (long long)a * P.o_h + lane * E);
@@ -322,24 +362,13 @@ paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
 }  // namespace
 
 int launch_plan(const Params& P, const Config& c, const PlanView& pv, cudaStream_t stream) {
-  paged_plan_kernel<<<1, kPlanThreads, 0, stream>>>(P, c, pv);
-  return check_launch("pa_paged_plan");
+  return launch_after("pa_paged_plan", paged_plan_kernel, 1, kPlanThreads, 0, stream, P, c, pv);
 }
 
 int launch_join(const Params& P, bool bf16, int D, const PlanView& pv, const Config& c,
                 const float* scratch, int sms, cudaStream_t stream) {
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(sms * 4);
-  cfg.blockDim = dim3(kJoinWarps * 32);
-  cfg.stream = stream;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  auto go = [&](auto kernel) -> int {
-    PA_CUDA(cudaLaunchKernelEx(&cfg, kernel, P, c, pv, scratch), "pa_paged_attn");
-    return PA_OK;
+  auto go = [&](auto kernel) {
+    return launch_after("pa_paged_attn", kernel, sms * 4, kJoinWarps * 32, 0, stream, P, c, pv, scratch);
   };
   if (D == 128) return bf16 ? go(paged_join_kernel<128, true>) : go(paged_join_kernel<128, false>);
   return bf16 ? go(paged_join_kernel<64, true>) : go(paged_join_kernel<64, false>);

@@ -65,6 +65,8 @@ __device__ __forceinline__ int find_request(const int2* pre, int n, int x, bool 
 __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(pa_paged_step_args a) {
   extern __shared__ int2 pre[];          // [requests + 1]: (tokens, pages) before request b
   __shared__ int2 warp_sum[kStepThreads / 32];
+  pdl_wait();
+  pdl_begin_next();
   const int B = a.requests, P = a.page_size;
   const long long W = a.table_width;
   auto div_up = [P](long long x) { return (x + P - 1) / P; };
@@ -149,6 +151,8 @@ constexpr int kAppendRows = 2;
 
 __global__ void __launch_bounds__(kAppendThreads)
 paged_append_kernel(pa_paged_append_args a, int vecs, int tpc) {
+  pdl_wait();
+  pdl_begin_next();
   // thread -> (token of the CTA's group, vector of the token's kv_heads * D elements)
   const int slots = a.pages * a.page_size;
   const int hv = a.D / 8;
@@ -209,8 +213,8 @@ extern "C" int pa_paged_step(const pa_paged_step_args* a, pa_stream_t stream) {
                                  smem), "pa_paged_step");
   int grid = (a->tokens + kStepThreads - 1) / kStepThreads;
   grid = grid < 1 ? 1 : grid > 148 ? 148 : grid;
-  paged_step_kernel<<<grid, kStepThreads, smem, (cudaStream_t)stream>>>(*a);
-  return check_launch("pa_paged_step");
+  return launch_after("pa_paged_step", paged_step_kernel, grid, kStepThreads, smem,
+                      (cudaStream_t)stream, *a);
 }
 
 extern "C" int pa_paged_append(const pa_paged_append_args* a, pa_stream_t stream) {
@@ -241,6 +245,6 @@ extern "C" int pa_paged_append(const pa_paged_append_args* a, pa_stream_t stream
   const int tpc = vecs >= kAppendThreads ? 1 : kAppendThreads / vecs;
   const int per = tpc * kAppendRows;
   const int grid = (a->tokens + per - 1) / per;
-  paged_append_kernel<<<grid, kAppendThreads, 0, (cudaStream_t)stream>>>(*a, vecs, tpc);
-  return check_launch("pa_paged_append");
+  return launch_after("pa_paged_append", paged_append_kernel, grid, kAppendThreads, 0,
+                      (cudaStream_t)stream, *a, vecs, tpc);
 }
