@@ -194,7 +194,7 @@ __host__ __device__ constexpr size_t slot_floats(int unit_rows) {
 
 // Keys of a unit whose rows sit at positions [i0, i1]: two runs of `cnt` keys a, a + step,
 // ..., of which those before `lo` are only there because a run with step 1 starts at a
-// multiple of the block.  A single position's lattice keys are listed one by one (step = the
+// multiple of `align` (a power of two, the rows that are copied together).  A single position's lattice keys are listed one by one (step = the
 // modulus), so that only they are read (not if kDense).  `exact`: every listed key from
 // lo on is live for every row.
 struct Runs {
@@ -202,7 +202,7 @@ struct Runs {
   bool exact;
 };
 template <int kBlock, bool kDense>
-__device__ __forceinline__ Runs unit_runs(const Pred& p, int i0, int i1, int len) {
+__device__ __forceinline__ Runs unit_runs(const Pred& p, int i0, int i1, int len, int align) {
   Runs r;
   r.step[0] = r.step[1] = 1;
   r.exact = i0 == i1;
@@ -217,7 +217,7 @@ __device__ __forceinline__ Runs unit_runs(const Pred& p, int i0, int i1, int len
     r.step[0] = p.mod;
     r.cnt[0] = i0 >= 0 && last >= first ? (last - first) / p.mod + 1 : 0;
     r.lo[1] = max(i0 - near + 1, 0);
-    r.a[1] = r.lo[1] & ~(kBlock - 1);
+    r.a[1] = r.lo[1] & ~(align - 1);
     r.cnt[1] = near > 0 ? max(top + 1 - r.a[1], 0) : 0;
     return r;
   }
@@ -225,11 +225,12 @@ __device__ __forceinline__ Runs unit_runs(const Pred& p, int i0, int i1, int len
   const KeyRanges k = key_ranges(p, i0, i1, len);
   r.lo[0] = k.a0;
   r.lo[1] = k.a1;
-  r.a[0] = k.a0 & ~(kBlock - 1);
-  r.a[1] = k.a1 & ~(kBlock - 1);
+  r.a[0] = k.a0 & ~(align - 1);
+  r.a[1] = k.a1 & ~(align - 1);
   r.cnt[0] = k.b0 > k.a0 ? k.b0 - r.a[0] : 0;
   r.cnt[1] = k.b1 > k.a1 ? k.b1 - r.a[1] : 0;
-  if (r.cnt[0] > 0 && r.cnt[1] > 0 && r.a[1] < k.b0) {   // they meet in one block: one run
+  // the first run's last block reaches into the second: one run
+  if (r.cnt[0] > 0 && r.cnt[1] > 0 && r.a[1] < r.a[0] + (r.cnt[0] + kBlock - 1) / kBlock * kBlock) {
     r.cnt[0] = k.b1 - r.a[0];
     r.cnt[1] = 0;
     r.exact = false;

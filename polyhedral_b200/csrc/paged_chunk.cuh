@@ -295,7 +295,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           u.n = min(R.n - at.t * per, per);
           u.pos0 = R.pos0 + at.t * per;
           u.len = R.len;
-          u.runs = unit_runs<128, true>(P.pred, u.pos0, u.pos0 + u.n - 1, u.len);
+          u.runs = unit_runs<128, true>(P.pred, u.pos0, u.pos0 + u.n - 1, u.len, C.seg);
           const int nblk = run_blocks<128>(u.runs);
           u.blk0 = fresh ? min(first.blk, nblk) : 0;
           u.blk1 = last ? min(end.blk, nblk) : nblk;

@@ -148,7 +148,7 @@ paged_few_kernel(const __grid_constant__ Params P, const Share* __restrict__ sha
     const int t0 = c.row0 / G, in0 = c.row0 - t0 * G;      // first token, head inside it
     auto token = [&](int r) { return t0 + div_group(P, in0 + r); };
     const int i0 = c.R.pos0 + t0, i1 = c.R.pos0 + token(c.rows - 1);
-    c.runs = unit_runs<kFewBlock, false>(P.pred, i0, i1, c.R.len);
+    c.runs = unit_runs<kFewBlock, false>(P.pred, i0, i1, c.R.len, kFewBlock);
     const int nblk = run_blocks<kFewBlock>(c.runs);
     c.blk0 = fresh ? min(first.blk, nblk) : 0;
     c.blk1 = last ? min(end.blk, nblk) : nblk;

@@ -17,11 +17,13 @@ __device__ __forceinline__ int unit_cost(const Params& P, const Config& c, const
   if (c.half_tokens) {
     const int t0 = t * 2 * c.half_tokens;
     return kUnitCost + run_blocks<128>(unit_runs<128, true>(
-                           P.pred, R.pos0 + t0, R.pos0 + min(R.n, t0 + 2 * c.half_tokens) - 1, R.len));
+                           P.pred, R.pos0 + t0, R.pos0 + min(R.n, t0 + 2 * c.half_tokens) - 1, R.len,
+                           min(1 << P.page_shift, 128)));
   }
   const int row0 = t * kFewRows, rows = min(R.n * P.group - row0, kFewRows);
   return kUnitCost + run_blocks<kFewBlock>(unit_runs<kFewBlock, false>(
-                         P.pred, R.pos0 + row0 / P.group, R.pos0 + (row0 + rows - 1) / P.group, R.len));
+                         P.pred, R.pos0 + row0 / P.group, R.pos0 + (row0 + rows - 1) / P.group, R.len,
+                         kFewBlock));
 }
 // Rows of a request's largest unit that hold a token.
 __device__ __forceinline__ int unit_rows_used(const Params& P, const Config& c, const Request& R) {
