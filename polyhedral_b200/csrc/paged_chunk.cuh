@@ -486,7 +486,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           ++tq[h];
         }
         uint32_t ks = 0, vs = 0;
-        bool started[2] = {false, false}, held[2] = {false, false};   // O begun; P V owed
+        // O begun; P V owed; no scores to come
+        bool started[2] = {false, false}, held[2] = {false, false}, last[2] = {false, false};
         // step u: the products with V of super-tile u - 1, then S of super-tile u
         for (int u = 0; u <= tiles && ok; ++u) {
           if (u > 0 && !(ok = wait_kv(vs))) break;
@@ -499,10 +500,18 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             if (held[h]) {
               if (!(ok = issue_pv(h, vs, started[h]))) break;
               started[h] = true;
+              if (last[h]) commit(&o_full[h]);
             }
+            // a piece may also end on super-tiles that the half skips for another reason
+            // (they are before its window)
+            if (u == tiles && started[h] && !last[h]) commit(&o_full[h]);
             held[h] = u < tiles && tile_live(ht[h], kb, sink_end);
-            if (held[h]) issue_s(h, ks);
-            if (u == tiles && started[h]) commit(&o_full[h]);
+            if (held[h]) {
+              issue_s(h, ks);
+              // a half whose last position is before the next super-tile is done with its
+              // scores: it need not wait for the other's last ones to write its result
+              last[h] = u == tiles - 1 || (blk + 1 < n0 ? kb + 128 : a1 + (blk + 1 - n0) * 128) > ht[h].i_hi;
+            }
           }
           if (!ok) break;
           if (u > 0) commit(&kv_empty[vs]);

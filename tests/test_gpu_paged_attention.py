@@ -57,6 +57,19 @@ def test_long_contexts_are_split(old, new, hint, spec):
     C.check(c, spec, o, lse)
 
 
+@pytest.mark.parametrize("old,new", [(3000, 900), (2945, 1000), (2900, 1055), (500, 1210), (0, 1300)])
+@pytest.mark.parametrize("spec", [(C.SINKS, 300, 4, 0), (C.SINKS, 1, 70, 0), (C.WINDOW, 257, 0, 0),
+                                  (C.TWOBAND, 100, 400, 60), (C.CAUSAL, 0, 0, 0)])
+def test_shares_cut_units_anywhere(old, new, spec):
+    """Enough units that the shares' cuts fall on every super-tile of some unit, super-tiles
+    that one half skips among them; twice the same bits."""
+    c = C.make([old, 17], [new, 40], 24, 24, 64, 64, BF, seed=9)
+    o, lse = C.run(c, spec)
+    C.check(c, spec, o, lse)
+    o2, lse2 = C.run(c, spec)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+
+
 @pytest.mark.parametrize("spec", [(C.WINDOW, 0, 0, 0), (C.FAR_STRIDED, 10**6, 4, 0),
                                   (C.SINKS, 0, 0, 0)])
 @pytest.mark.parametrize("lens", [DECODE, MIXED], ids=["decode", "mixed"])
