@@ -18,12 +18,13 @@ Everything is stream-ordered and nothing is read back by the host, so a step of 
 shapes can be captured in a CUDA graph.  The reference has no counterpart.
 """
 import ctypes
+import functools
 
 import torch
 
 from . import _lib
 
-_current_device = torch.cuda.current_device
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 _DTYPES = {torch.bfloat16: _lib.PA_BF16, torch.float16: _lib.PA_F16}
@@ -174,8 +175,26 @@ def append_kv(k, v, k_cache, v_cache, slot_map):
         raise ValueError("k and v: last dimension must be contiguous")
     args = _pack_append(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                         _int32("slot_map", slot_map, T, dev), T, H, D, pages, page_size,
-                        kt, kh, vt, vh, *ks[:3], *vs[:3])
+                        kt, kh, vt, vh, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
     _launch("pa_paged_append", dev, args)
+
+
+def _plan_args(head, tail, seq_lens, q_start):
+    """Arguments of the plan's calls: there is no table yet, lengths are what seq_lens says."""
+    B, T, H, Hkv, D, page, max_new, max_len = head
+    return _pack_attn(0, 0, 0, 0, 0, 0, seq_lens, q_start, B, T, H, Hkv, D, 0, 0, page,
+                      2**24 // page if page > 0 else 1, max_new, max_len, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                      0, 0, 0, *tail, 0.0)
+
+
+@functools.lru_cache(maxsize=256)
+def _plan_sizes(head, device):
+    """Bytes of a plan and of one call's scratch for these sizes on that device (they follow
+    from the sizes and the number of multiprocessors)."""
+    lib = _lib.load()
+    args = _plan_args(head, (0, 0, 0, 0), 256, 256)
+    with _lib.on_device(device):
+        return max(lib.pa_paged_plan_size(args), 256), lib.pa_paged_scratch_size(args)
 
 
 class PagedPlan:
@@ -189,17 +208,11 @@ class PagedPlan:
     def __init__(self, seq_lens, q_start, head, tail, key, device):
         self.seq_lens, self.q_start, self.key = seq_lens, q_start, key
         self.head, self.tail, self.device = head, tail, device
-        # no table here: lengths are what seq_lens says
-        B, T, H, Hkv, D, page, max_new, max_len = head
-        args = _pack_attn(0, 0, 0, 0, 0, 0, seq_lens.data_ptr(), q_start.data_ptr(), B, T, H, Hkv,
-                          D, 0, 0, page, max(2**24 // max(page, 1), 1), max_new, max_len,
-                          *(0,) * 12, *tail, 0.0)
-        lib = _lib.load()
-        with _lib.on_device(device):                 # sizes follow the device's multiprocessors
-            self.nbytes = lib.pa_paged_plan_size(args)
-            self.scratch_bytes = lib.pa_paged_scratch_size(args)
-        self.buffer = torch.empty(max(self.nbytes, 256), dtype=torch.uint8, device=seq_lens.device)
-        _launch("pa_paged_plan", device, args, self.buffer.data_ptr(), self.nbytes)
+        self.nbytes, self.scratch_bytes = _plan_sizes(head, device)
+        self.buffer = torch.empty(self.nbytes, dtype=torch.uint8, device=seq_lens.device)
+        _launch("pa_paged_plan", device,
+                _plan_args(head, tail, seq_lens.data_ptr(), q_start.data_ptr()),
+                self.buffer.data_ptr(), self.nbytes)
 
     def status(self):
         """Device status of the forwards on this plan so far (synchronises): 0, or the code
@@ -227,9 +240,8 @@ def make_plan(seq_lens, q_start, kind, p0, p1, p2, *, tokens, heads, kv_heads, h
     _int32("seq_lens", seq_lens, B, dev)
     _int32("q_start", q_start, B + 1, dev)
     return PagedPlan(seq_lens, q_start,
-                     (B, int(tokens), int(heads), int(kv_heads), int(head_dim), int(page_size),
-                      int(max_new), int(max_len)),
-                     (int(kind), int(p0), int(p1), int(p2)),
+                     (B, tokens, heads, kv_heads, head_dim, page_size, max_new, max_len),
+                     (kind, p0, p1, p2),
                      (B, tokens, heads, kv_heads, head_dim, page_size, kind, p0, p1, p2), dev)
 
 
@@ -303,14 +315,14 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, q_start, kind, p
     elif return_lse:
         lse = torch.empty(H, T, dtype=torch.float32, device=device)
         lse_row, lse_ptr = T, lse.data_ptr()
-    scratch, nbytes, scratch_ptr = None, plan.scratch_bytes, 0
+    head, scratch, nbytes, scratch_ptr = plan.head, None, plan.scratch_bytes, 0
     if nbytes:
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
         scratch_ptr = scratch.data_ptr()
     args = _pack_attn(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), lse_ptr,
                       block_table.data_ptr(), lens_ptr, start_ptr, B, T, H, Hkv, D, _DTYPES[dtype],
-                      pages, page_size, width, *plan.head[6:], row, qt, qh, *ks[:3], *vs[:3], ot, oh,
-                      lse_row, *plan.tail, scale or 0.0)
+                      pages, page_size, width, head[6], head[7], row, qt, qh, ks[0], ks[1], ks[2], vs[0],
+                      vs[1], vs[2], ot, oh, lse_row, kind, p0, p1, p2, scale or 0.0)
     _launch("pa_paged_attn", dev, args, plan.buffer.data_ptr(), plan.nbytes, scratch_ptr, nbytes)
     if check:
         st = plan.status()
