@@ -242,9 +242,14 @@ paged_plan_kernel(const __grid_constant__ Params P, Config c, PlanView pv) {
 }
 
 // One divided unit's row: O = sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i over its pieces, m
-// the largest m_i.  A warp joins a row, or, where units have many pieces, the CTA's warps
-// share them out.  (The order of `cuts` is that of an atomic counter; it decides only which
-// CTA joins which unit.)
+// the largest m_i.  Reading the pieces bounds it (they are in L2).  Three ways, by how many
+// rows and pieces there are: of the chunk kernel's large units a warp takes 8 rows, 4 at a time
+// so that their loads overlap and the unit's addresses are worked out once (a row per warp
+// was bound by those instructions: 24 ragged requests took 104 us in all instead of 96); of
+// the few-rows kernel's small ones a warp takes one row, four pieces at a time (8 rows as
+// above: 64 requests' decode took 163 us instead of 158); and where units have many pieces
+// the warps of a CTA share a row's.  (The order of `cuts` is that of an atomic counter; it
+// decides only which warp joins which row.)
 constexpr int kJoinWarps = 8;
 
 template <int D, bool kBf16>
@@ -259,37 +264,109 @@ paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
   pdl_begin_next();
   const int used = pv.meta[0], cuts = pv.meta[1], rows = pv.meta[2];
   const bool many = used > kJoinWarps * cuts;   // pieces per unit, on average
-  const int items = cuts * rows;
   const int unit_rows = c.unit_rows;
   const size_t slot = slot_floats<D>(unit_rows);
-  const int first = many ? blockIdx.x : blockIdx.x * kJoinWarps + warp;
-  const int step = many ? gridDim.x : gridDim.x * kJoinWarps;
-  for (int it = first; it < items; it += step) {
-    const Cut cut = pv.cuts[it / rows];
-    const int w0 = cut.worker, pieces = cut.pieces, r = it % rows;
-    const Request R = cut.R;
-    int tok, g;                                  // token of the request, head of the group
-    bool there;
+  const float* ml0 = scratch + (size_t)unit_rows * D;
+  // row r of a unit: its token of the request (-1: none) and head of the group
+  auto place = [&](const Cut& cut, int r, int& g) -> int {
+    int t;
     if (c.half_tokens) {
-      const int x = r & 127;
-      tok = x / P.group;
-      g = x - tok * P.group;
-      there = tok < c.half_tokens;
-      tok += (cut.t * 2 + (r >> 7)) * c.half_tokens;
-      there = there && tok < R.n;
+      const int x = r & 127, y = div_group(P, x);
+      g = x - y * P.group;
+      t = y < c.half_tokens ? (cut.t * 2 + (r >> 7)) * c.half_tokens + y : -1;
     } else {
       const int row = cut.t * kFewRows + r;
-      tok = row / P.group;
-      g = row - tok * P.group;
-      there = tok < R.n;
+      t = row / P.group;
+      g = row - t * P.group;
     }
-    if (!there) continue;                        // alike for the whole CTA, where it shares a row
+    return t < cut.R.n ? t : -1;
+  };
+  auto write = [&](const Cut& cut, int tok, int g, float m, float l, const float (&acc)[E]) {
+    const int t = cut.R.row0 + tok, a = cut.h * P.group + g;
+    const float inv = l == 0.f ? 0.f : 1.f / l;   // a sum that is no number stays one
+    uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(P.o) + (long long)t * P.o_t +
+                                              (long long)a * P.o_h + lane * E);
+    if constexpr (E == 4)
+      *reinterpret_cast<uint2*>(o) = make_uint2(pack_pair<kBf16>(acc[0] * inv, acc[1] * inv),
+                                                pack_pair<kBf16>(acc[2] * inv, acc[3] * inv));
+    else
+      o[0] = pack_pair<kBf16>(acc[0] * inv, acc[1] * inv);
+    if (P.lse && lane == 0)
+      P.lse[a * P.lse_h + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+  };
+  auto load = [&](size_t at, int r, float2& ml, float (&x)[E]) {
+    ml = *reinterpret_cast<const float2*>(ml0 + at + 2 * r);
+    if constexpr (E == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(scratch + at + (size_t)r * D + lane * 4);
+      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(scratch + at + (size_t)r * D + lane * 2);
+      x[0] = v.x; x[1] = v.y;
+    }
+  };
+  constexpr int U = 4;
+
+  if (!many && c.half_tokens) {
+    constexpr int kGroup = 8;
+    const int groups = (rows + kGroup - 1) / kGroup;
+    for (int it = blockIdx.x * kJoinWarps + warp; it < cuts * groups; it += gridDim.x * kJoinWarps) {
+      const int k = it / groups;
+      const Cut cut = pv.cuts[k];
+      const int r0 = (it - k * groups) * kGroup;
+#pragma unroll 1
+      for (int r1 = r0; r1 < r0 + kGroup; r1 += U) {
+        int tok[U], g[U];
+        float m[U], l[U], acc[U][E];
+        bool some = false;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          tok[u] = r1 + u < unit_rows ? place(cut, r1 + u, g[u]) : -1;
+          some |= tok[u] >= 0;
+          m[u] = -INFINITY;
+          l[u] = 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[u][e] = 0.f;
+        }
+        if (!some) continue;
+#pragma unroll 1
+        for (int p = 0; p < cut.pieces; ++p) {
+          const size_t at = (size_t)(p == 0 ? 2 * cut.worker + 1 : 2 * (cut.worker + p)) * slot;
+          float2 ml[U];
+          float x[U][E];
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (tok[u] >= 0) load(at, r1 + u, ml[u], x[u]);
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            if (tok[u] < 0) continue;
+            const float mn = fmaxf(m[u], ml[u].x), z = mn == -INFINITY ? 0.f : mn;
+            const float f = ex2f(m[u] - z), h = ex2f(ml[u].x - z);
+            m[u] = mn;
+            l[u] = fmaf(h, ml[u].y, l[u] * f);
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[u][e] = fmaf(h, x[u][e], acc[u][e] * f);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (tok[u] >= 0) write(cut, tok[u], g[u], m[u], l[u], acc[u]);
+      }
+    }
+    return;
+  }
+
+  const int it0 = many ? blockIdx.x : blockIdx.x * kJoinWarps + warp;
+  for (int it = it0; it < cuts * rows; it += many ? gridDim.x : gridDim.x * kJoinWarps) {
+    const int k = it / rows, r = it - k * rows;
+    const Cut cut = pv.cuts[k];
+    int g;
+    const int tok = place(cut, r, g);
+    if (tok < 0) continue;                       // alike for the whole CTA, where it shares a row
     float m = -INFINITY, l = 0.f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    const int p0 = many ? warp : 0, dp = many ? kJoinWarps : 1;
-    constexpr int U = 4;
-    for (int p = p0; p < pieces; p += dp * U) {
+    const int dp = many ? kJoinWarps : 1;
+    for (int p = many ? warp : 0; p < cut.pieces; p += dp * U) {
       float2 ml[U];
       float x[U][E];
 #pragma unroll
@@ -298,17 +375,8 @@ paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
         ml[u] = make_float2(-INFINITY, 0.f);
 #pragma unroll
         for (int e = 0; e < E; ++e) x[u][e] = 0.f;
-        if (q < pieces) {
-          const float* s = scratch + (size_t)(q == 0 ? 2 * w0 + 1 : 2 * (w0 + q)) * slot;
-          ml[u] = *reinterpret_cast<const float2*>(s + (size_t)unit_rows * D + 2 * r);
-          if constexpr (E == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(s + (size_t)r * D + lane * 4);
-            x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
-          } else {
-            const float2 v = *reinterpret_cast<const float2*>(s + (size_t)r * D + lane * 2);
-            x[u][0] = v.x; x[u][1] = v.y;
-          }
-        }
+        if (q < cut.pieces)
+          load((size_t)(q == 0 ? 2 * cut.worker + 1 : 2 * (cut.worker + q)) * slot, r, ml[u], x[u]);
       }
       float mn = m;
 #pragma unroll
@@ -321,10 +389,10 @@ paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
       for (int e = 0; e < E; ++e) acc[e] *= f;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float g = ex2f(ml[u].x - z);
-        l = fmaf(g, ml[u].y, l);
+        const float h = ex2f(ml[u].x - z);
+        l = fmaf(h, ml[u].y, l);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(g, x[u][e], acc[e]);
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(h, x[u][e], acc[e]);
       }
     }
     if (many) {
@@ -338,26 +406,19 @@ paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
 #pragma unroll
       for (int i = 0; i < kJoinWarps; ++i) mn = fmaxf(mn, s_ml[i].x);
       const float z = mn == -INFINITY ? 0.f : mn;
-      m = mn;
       l = 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] = 0.f;
 #pragma unroll
       for (int i = 0; i < kJoinWarps; ++i) {
-        const float g = ex2f(s_ml[i].x - z);
-        l = fmaf(g, s_ml[i].y, l);
+        const float h = ex2f(s_ml[i].x - z);
+        l = fmaf(h, s_ml[i].y, l);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(g, s_acc[i][lane * E + e], acc[e]);
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(h, s_acc[i][lane * E + e], acc[e]);
       }
+      m = mn;
     }
-    const int t = R.row0 + tok, a = cut.h * P.group + g;
-    const float inv = l == 0.f ? 0.f : 1.f / l;   // a sum that is no number stays one
-    uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(P.o) + (long long)t * P.o_t +
-                                              (long long)a * P.o_h + lane * E);
-#pragma unroll
-    for (int e = 0; e < E; e += 2) o[e / 2] = pack_pair<kBf16>(acc[e] * inv, acc[e + 1] * inv);
-    if (P.lse && lane == 0)
-      P.lse[a * P.lse_h + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+    write(cut, tok, g, m, l, acc);
   }
 }
 
