@@ -207,6 +207,21 @@ extern "C" int pa_paged_step(const pa_paged_step_args* a, pa_stream_t stream) {
                    ((a->slot_map && a->positions) || a->tokens == 0),
                "pa_paged_step: null pointer");
   PA_CHECK_ARG(a->free_head != a->free_head_out, "pa_paged_step: free_head_out is free_head");
+  // every CTA reads the inputs while one of them writes the outputs
+  struct Span {
+    const int32_t* p;
+    long long n;
+  };
+  const long long B = a->requests;
+  const Span in[] = {{a->old_lens, B}, {a->new_lens, B}, {a->free_pages, a->free_count},
+                     {a->free_head, 1}};
+  const Span out[] = {{a->q_start, B + 1}, {a->seq_lens, B}, {a->slot_map, a->tokens},
+                      {a->positions, a->tokens}, {a->free_head_out, 1}, {a->missing, 1},
+                      {a->block_table, (B - 1) * a->table_stride + a->table_width}};
+  for (const Span& x : in)
+    for (const Span& y : out)
+      PA_CHECK_ARG(x.n == 0 || y.n == 0 || x.p + x.n <= y.p || y.p + y.n <= x.p,
+                   "pa_paged_step: an output overlaps old_lens, new_lens, free_pages or free_head");
   const int smem = (a->requests + 1) * (int)sizeof(int2);
   if (smem > 40 * 1024)
     PA_CUDA(cudaFuncSetAttribute(paged_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,

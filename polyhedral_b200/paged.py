@@ -109,8 +109,9 @@ def make_step(block_table, old_lens, new_lens, free_pages, free_head, *, page_si
     ``old_lens + new_lens`` tokens need more pages gets them from ``free_pages``, from entry
     ``free_head`` [1] on, requests in order; no other entry is touched.  ``tokens`` is the
     capacity of the slot map (at least the sum of ``new_lens``).  ``out`` (a
-    ``PagedStep`` of the same sizes) is filled instead of a new one; its ``free_head``
-    must not be the one given.  All arguments are int32 tensors on one CUDA device; at most
+    ``PagedStep`` of the same sizes) is filled instead of a new one; none of its tensors may
+    be an argument too (the next step's ``old_lens`` is this one's ``seq_lens``: use two
+    in turn).  All arguments are int32 tensors on one CUDA device; at most
     16384 requests."""
     B, width, row = _table(block_table, "make_step")
     dev = block_table.get_device()

@@ -32,10 +32,9 @@ def test_struct_layout_matches_header(cname, pyname):
 
 def _step_args():
     a = _lib.PaPagedStepArgs()
-    for name, kind in a._fields_:
+    for i, (name, kind) in enumerate(a._fields_):
         if kind is _lib.c_vp:
-            setattr(a, name, 256)
-    a.free_head_out = 512
+            setattr(a, name, 4096 * i)
     a.requests, a.page_size, a.table_width, a.tokens, a.free_count, a.table_stride = 4, 16, 8, 4, 9, 8
     return a
 
@@ -45,10 +44,16 @@ def _step_args():
     ("page_size", 0, b"page_size=0"), ("table_width", 0, b"table_width=0"),
     ("tokens", -1, b"tokens=-1"), ("free_count", -1, b"free_count=-1"),
     ("table_stride", 7, b"table_stride=7"), ("old_lens", None, b"null"),
-    ("slot_map", None, b"null"), ("free_head_out", 256, b"free_head_out")])
+    ("slot_map", None, b"null"), ("free_head_out", "free_head", b"free_head_out"),
+    ("seq_lens", "old_lens", b"overlaps"), ("old_lens", "q_start", b"overlaps"),
+    ("positions", "new_lens", b"overlaps"), ("free_pages", "block_table", b"overlaps")])
 def test_step_refusals(lib, field, value, word):
     a = _step_args()
-    setattr(a, field, value)
+    # a name: the same memory as that argument's, from its second entry on
+    same = getattr(a, value) if isinstance(value, str) else value
+    if isinstance(value, str) and field != "free_head_out":
+        same += 4
+    setattr(a, field, same)
     assert lib.pa_paged_step(ctypes.byref(a), None) == _lib.PA_ERR_ARG
     assert word in lib.pa_last_error()
 
