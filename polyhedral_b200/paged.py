@@ -14,8 +14,9 @@ and its *slot* is ``page * page_size + row``.  One step of a serving loop:
                                   step.q_start, *mask.spec, plan=plan)
     free_head = step.free_head
 
-Everything is stream-ordered and nothing is read back by the host, so a step of fixed
-shapes can be captured in a CUDA graph.  The reference has no counterpart.
+There are no gradients: these serve.  Everything is stream-ordered and nothing is read
+back by the host, so a step of fixed shapes can be captured in a CUDA graph.  The reference
+has no counterpart.
 """
 import ctypes
 import functools

@@ -265,3 +265,24 @@ def test_wide_masks():
         for hint in (0, 1):
             o, lse = C.run(c, spec, max_new=hint)
             C.check(c, (C.CAUSAL, 0, 0, 0), o, lse)
+
+
+@pytest.mark.parametrize("lens", [([300, 70], [1, 1]), ([200, 33], [90, 40])])
+def test_parts_join_with_lse_merge(lens):
+    """Disjoint masks over one cache (the near band, everything behind it) joined by
+    ``merge.lse_merge`` are the causal attention: each part is within its bound, and the
+    merge rounds once more, so 2.5 bounds cover the three."""
+    from polyhedral_b200 import merge
+    c = C.make(*lens, 8, 2, 128, 16, BF, seed=14)
+    parts = [C.run(c, spec) for spec in ((C.WINDOW, 40, 0, 0), (C.FAR_STRIDED, 40, 1, 0))]
+    (o1, l1), (o2, l2) = ((o.transpose(0, 1), lse) for o, lse in parts)
+    o, lse = merge.lse_merge(o1, l1, o2, l2)
+    spec = (C.CAUSAL, 0, 0, 0)
+    o_ref, lse_ref = PO.paged_attention(c["q"], c["k_cache"], c["v_cache"], c["block_table"],
+                                        c["seq_lens"], c["q_start"], *spec)
+    bo, bl = C.bounds(c, spec, o_ref)
+    # a part's own mean of |v| may exceed the whole's: 4 bounds |v| < 4 as well
+    bo = 2.5 * (bo + 2.0**-7 * 4.0 * 0.25)
+    err = (o.transpose(0, 1).double().cpu() - o_ref).abs()
+    assert (err <= bo).all(), float((err / bo).max())
+    assert (lse.double().cpu() - lse_ref).abs().max() <= 2.5 * bl
