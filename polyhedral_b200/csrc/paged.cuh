@@ -158,6 +158,7 @@ struct Config {
   int half_tokens;    // chunk kernel: tokens per half of a unit; few-rows kernel: 0
   int workers;        // most shares
   int min_share;      // blocks below which a share is not worth a worker
+  int min_piece;      // blocks of a piece below which a unit is not cut there
   int split;          // units may be cut
 };
 

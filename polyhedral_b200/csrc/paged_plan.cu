@@ -190,10 +190,13 @@ paged_plan_kernel(const __grid_constant__ Params P, Config c, PlanView pv) {
       }
     }
     if (in) {
-      // a cut inside the unit's own cost, or where units stay whole, falls on its begin --
-      // or, units staying whole, on the next unit's for all but its first cut
+      // A cut inside the unit's own cost, or so early that the piece before it would be short,
+      // falls on the unit's begin; one that would leave a short piece behind it, or any
+      // inside a unit where units stay whole, on the next unit's.
       sh.blk = max((int)rem - kUnitCost, 0);
-      if (!c.split && rem > 0) {
+      if (sh.blk < c.min_piece) sh.blk = 0;
+      const int left = unit_cost(P, c, R, sh.t) - kUnitCost - sh.blk;
+      if (c.split ? sh.blk > 0 && left < c.min_piece : rem > 0) {
         sh.blk = 0;
         if (++sh.t >= n) {
           sh.t = 0;
