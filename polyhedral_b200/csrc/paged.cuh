@@ -162,7 +162,8 @@ struct Config {
   int split;          // units may be cut
 };
 
-// Blocks that a unit costs beside its own (loading q, writing o).
+// Blocks that a unit costs beside its own (loading q, writing o): 24 ragged requests took 97
+// us with 2 or 3, 101 us with 1.
 constexpr int kUnitCost = 2;
 
 struct PlanView {

@@ -612,7 +612,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             }
             if (P.pred.kind == PA_LOCAL_STRIDED || P.pred.kind == PA_DILATED) a0 = 0;   // every key
             if (P.pred.kind == PA_FAR_STRIDED) b0 = min(c - P.pred.p0, c);
-            if (whole) {
+            if (whole && kb >= g.w && P.pred.kind != PA_TWOBAND) {   // one range
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mk[k] = range_bits(a0, b0, k * 32);
+            } else if (whole) {
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 mk[k] = range_bits(a0, b0, k * 32) | range_bits(a1, b1, k * 32);
@@ -677,10 +680,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         }
         if (__builtin_expect(!full, 0)) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
+          for (int k = 0; k < 4; ++k) {
 #pragma unroll
             for (int x = 0; x < 32; ++x)
               if (!((mk[k] >> x) & 1u)) s[k * 32 + x] = -INFINITY;
+          }
         }
         float mx;
         {
