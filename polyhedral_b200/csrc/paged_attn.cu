@@ -97,7 +97,16 @@ Config choose(const pa_paged_attn_args* a, int sms) {
   Config c;
   const int group = a->heads / a->kv_heads;
   const long long most = a->max_new > 0 && a->max_new < a->tokens ? a->max_new : a->tokens;
-  if (most * group <= kFewRows) {
+  // Few rows: the keys are read once and bound the work (64 requests' decode: 165 us; through
+  // the chunk kernel 226 us; with 32 rows per key head, read twice, 331 us against 249 us).
+  // Few keys in all, at most 4 blocks a worker: latency bounds it, and the chunk kernel's is
+  // longer (64 tokens of one request: 13 us on the GPU against 20 us; 4 tokens after 999, 64
+  // query heads: 15 against 32 us; 16 requests of 16 after 500, 14 blocks a worker: 32
+  // against 24 us).
+  const long long units = (most * group + kFewRows - 1) / kFewRows * a->requests * a->kv_heads;
+  const long long each = (a->max_len + kFewBlock - 1ll) / kFewBlock;
+  const bool few_keys = a->max_len > 0 && units <= 4ll * sms * kFewWarps / each;
+  if (most * group <= kFewRows || few_keys) {
     c.unit_rows = kFewRows;
     c.half_tokens = 0;
     c.workers = sms * kFewWarps;
@@ -114,8 +123,8 @@ Config choose(const pa_paged_attn_args* a, int sms) {
     // anywhere, 24 us with pieces of 3; 22 requests of 356, 39 and 31 us
     c.min_piece = 3;
   }
-  // a request's keys that fit two shares are read by one warp sooner than by several
-  // and the join behind them
+  // Requests of at most 128 tokens stay whole, which spares the join: 8 requests of some 100
+  // tokens, 14.1 us a call instead of 18.0 us (on the GPU alone 14.3 us instead of 13.3 us).
   c.split = !(a->max_len > 0 && a->max_len <= 128);
   return c;
 }

@@ -27,6 +27,18 @@ def test_masks(spec, lens, dtype):
     C.check(c, spec, o, lse)
 
 
+@pytest.mark.parametrize("spec", SPECS)
+@pytest.mark.parametrize("lens,longest", [(([0, 33, 90, 0], [17, 5, 30, 0]), 120), (MIXED, 364)],
+                         ids=["short", "mixed"])
+@pytest.mark.parametrize("heads,kv_heads,D", [(4, 2, 64), (6, 2, 128), (24, 1, 64)])
+def test_small_chunks_with_known_lengths(spec, lens, longest, heads, kv_heads, D):
+    """With few keys in all the few-rows kernel takes chunks too, units that begin and end
+    inside a token among them."""
+    c = C.make(*lens, heads, kv_heads, D, 16, BF, seed=11)
+    o, lse = C.run(c, spec, max_new=max(lens[1]), max_len=longest)
+    C.check(c, spec, o, lse)
+
+
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (6, 2), (5, 5), (7, 1), (16, 2), (24, 2), (48, 2),
                                             (128, 1)])
 @pytest.mark.parametrize("D", [64, 128])
