@@ -1,4 +1,5 @@
-// Attention of few new tokens (one, as a rule) over a paged K/V cache.
+// Attention of few new tokens (one, as a rule) over a paged K/V cache, and of any where the
+// keys are few in all.
 //
 // With at most 16 query rows per key head the work is reading the cache: 4 D bytes per
 // key against 4 D FLOP per key and row, at most 16 FLOP per byte where the GPU has 250.  So HBM

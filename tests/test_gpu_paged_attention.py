@@ -173,3 +173,28 @@ def test_non_finite_values_in_masked_places(bad, lens):
             # the rows may be summed in another order now; each sum keeps the bound of
             # paged_cases.bounds (e + 2e-5, e = 1.3e-4), so two are within twice that
             assert (lse2 - lse)[:, : c["tokens"]].abs().max() <= 2 * (1.3e-4 + 2e-5)
+
+
+@pytest.mark.parametrize("old,new,hint", [([3000], [3], 3), ([2500, 60], [90, 1], 0)])
+def test_non_finite_values_in_split_requests(old, new, hint):
+    """The last token's value breaks down in a request that is divided among workers: only the
+    last row does; and a value that every row sees reaches all of them."""
+    spec = (C.CAUSAL, 0, 0, 0)
+    c = C.make(old, new, 4, 2, 128, 16, BF, seed=15)
+    o, lse = C.run(c, spec, max_new=hint)
+    C.check(c, spec, o, lse)
+    j = old[0] + new[0] - 1
+    t = c["block_table"][0].long()
+    c["v_cache"][t[j // 16], j % 16] = float("nan")
+    o2, lse2 = C.run(c, spec, max_new=hint)
+    last = new[0] - 1
+    assert torch.isnan(o2[last]).all() and torch.isfinite(o2[:last]).all()
+    assert torch.isfinite(o2[new[0]:]).all()
+    # both are within paged_cases.bounds of the same 64-bit result
+    bo, bl = C.bounds(c, spec, torch.zeros(o.shape, dtype=torch.float64))
+    tol = 2 * (bo[:last] + 2.0**-8 * o[:last].double().cpu().abs())
+    assert ((o2 - o).double().cpu().abs()[:last] <= tol).all()
+    assert (lse2 - lse).abs().max() <= 2 * bl
+    c["v_cache"][t[7], 3] = float("inf")
+    o3, _ = C.run(c, spec, max_new=hint)
+    assert torch.isinf(o3[:last]).all() and torch.isfinite(o3[new[0]:]).all()
