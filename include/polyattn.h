@@ -397,8 +397,9 @@ PA_API size_t pa_paged_scratch_size(const pa_paged_attn_args* args);
 
 /* Builds, in `plan`, the shares of work of the forward's CTAs from seq_lens and q_start
  * (read now, on `stream`) and the predicate.  The plan serves every forward with the same
- * lengths, sizes and predicate -- all layers of a step -- and is only read by them, so
- * they may run on several streams at once. */
+ * lengths, sizes and predicate -- all layers of a step -- and is only read by them (its
+ * status word apart, which a failing wait sets), so they may run on several streams at
+ * once. */
 PA_API int pa_paged_plan(const pa_paged_attn_args* args, void* plan, size_t plan_bytes,
                          pa_stream_t stream);
 
