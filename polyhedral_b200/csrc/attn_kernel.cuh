@@ -180,6 +180,13 @@ __device__ __forceinline__ void fma2v(float& d0, float& d1, float a0, float a1, 
       : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
 }
 
+// The larger of two values, NaN where either is one (fmaxf drops a NaN).
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
 // Pairs (index i = 0..15 of each 32-column chunk of a row) whose exponentials run on
 // the FMA pipe (exp2_fma) instead of the XU pipe.  On B200 ex2 is the softmax's only
 // XU instruction, at 8 cycles per warp instruction per scheduler: the exponentials of
@@ -200,12 +207,12 @@ constexpr uint32_t kFmaExpPairs = PA_FMA_EXP_PAIRS;
 // j + 127, made by one integer multiply-add on t's bits ((j mod 2^9) << 23 plus the
 // bits of 1.0f, mod 2^32).  x is clamped to >= -127 first, where that field is 0: the
 // scale is exactly 0, so a masked score (-inf) gives exactly 0, as ex2.approx.ftz
-// does.  Used for x <= 127 (the softmax's x never exceeds the lazy-rescale margin).
+// does; a NaN stays one.  Used for x <= 127 (the softmax's x never exceeds the lazy-rescale margin).
 __device__ __forceinline__ void exp2_fma(float x0, float x1, float& y0, float& y1) {
   constexpr float kRound = 12582912.0f;   // 1.5 * 2^23
   constexpr float kC0 = 0.99992811f, kC1 = 0.69326097f, kC2 = 0.24261054f, kC3 = 0.055171322f;
-  x0 = fmaxf(x0, -127.0f);
-  x1 = fmaxf(x1, -127.0f);
+  x0 = max_or_nan(x0, -127.0f);
+  x1 = max_or_nan(x1, -127.0f);
   float t0, t1, j0, j1, f0, f1, p0, p1;
   fma2v(t0, t1, x0, x1, 1.0f, 1.0f, kRound, kRound);        // t = x + R
   fma2v(j0, j1, t0, t1, 1.0f, 1.0f, -kRound, -kRound);      // j = t - R (exact)

@@ -146,11 +146,13 @@ __device__ __forceinline__ bool elect_one() {
 
 // 2^x for two values on the FMA and integer pipes: j = rint(x) by adding 1.5 * 2^23, 2^(x - j)
 // by a degree-4 polynomial fitted for least maximum relative error on [-1/2, 1/2] (2.7e-6 in
-// 32 bits), 2^j by its exponent field.  x <= 127; below -127, -inf too, the scale is 0.
+// 32 bits), 2^j by its exponent field.  x <= 127; below -127, -inf too, the scale is 0.  A
+// NaN stays one (a clamp by fmaxf would make it -127, and the key that it comes from would
+// drop out of the row).
 __device__ __forceinline__ void exp2_poly(float x0, float x1, float& y0, float& y1) {
   constexpr float kRound = 12582912.0f;
-  x0 = fmaxf(x0, -127.0f);
-  x1 = fmaxf(x1, -127.0f);
+  x0 = attn::max_or_nan(x0, -127.0f);
+  x1 = attn::max_or_nan(x1, -127.0f);
   float t0, t1, j0, j1, f0, f1, p0, p1;
   attn::fma2v(t0, t1, x0, x1, 1.0f, 1.0f, kRound, kRound);
   attn::fma2v(j0, j1, t0, t1, 1.0f, 1.0f, -kRound, -kRound);
