@@ -192,6 +192,18 @@ def call(name, *args, device=None):
     return rc
 
 
+def device_status(name, plan):
+    """Status word that the entry point `name` reads from a plan's buffer (synchronises the
+    current stream of its device): 0 or a device code.  Raises when it cannot be read -- a
+    CUDA error, of an earlier kernel too -- since the word says nothing then."""
+    lib, st = load(), c_i32(0)
+    with on_device(plan.device):
+        rc = getattr(lib, name)(plan.data_ptr(), ctypes.byref(st), stream_handle(plan.device))
+    if rc not in (PA_OK, PA_ERR_DEVICE):
+        raise PolyattnError(name, rc, lib.pa_last_error().decode(errors="replace"))
+    return int(st.value)
+
+
 def stream_handle(device=None):
     """Raw cudaStream_t of torch's current stream on `device`.  Read through torch's
     raw-stream accessor when it has one (no Stream object is built per call, which

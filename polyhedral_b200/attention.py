@@ -78,12 +78,7 @@ class AttnPlan:
     def status(self):
         """Device status of the most recent forward on this plan (synchronises): 0
         when it finished cleanly, else the code of the bounded wait that ran out."""
-        st = _lib.c_i32(0)
-        lib = _lib.load()
-        with _lib.on_device(self.workspace.device):
-            lib.pa_attn_status(self.workspace.data_ptr(), ctypes.byref(st),
-                               _lib.stream_handle(self.workspace.device))
-        return int(st.value)
+        return _lib.device_status("pa_attn_status", self.workspace)
 
 
 def _ptr(t):

@@ -18,7 +18,6 @@ There are no gradients: these serve.  Everything is stream-ordered and nothing i
 back by the host, so a step of fixed shapes can be captured in a CUDA graph.  The reference
 has no counterpart.
 """
-import ctypes
 import functools
 
 import torch
@@ -219,11 +218,7 @@ class PagedPlan:
     def status(self):
         """Device status of the forwards on this plan so far (synchronises): 0, or the code
         of the bounded wait that ran out."""
-        st = _lib.c_i32(0)
-        with _lib.on_device(self.device):
-            _lib.load().pa_paged_status(self.buffer.data_ptr(), ctypes.byref(st),
-                                        _lib.stream_handle(self.device))
-        return int(st.value)
+        return _lib.device_status("pa_paged_status", self.buffer)
 
 
 def make_plan(seq_lens, q_start, kind, p0, p1, p2, *, tokens, heads, kv_heads, head_dim,
