@@ -398,8 +398,9 @@ PA_API size_t pa_paged_scratch_size(const pa_paged_attn_args* args);
 /* Builds, in `plan`, the shares of work of the forward's CTAs from seq_lens and q_start
  * (read now, on `stream`) and the predicate.  The plan serves every forward with the same
  * lengths, sizes and predicate -- all layers of a step -- and is only read by them (its
- * status word apart, which a failing wait sets), so they may run on several streams at
- * once. */
+ * status word apart, which a failure sets), so they may run on several streams at once.
+ * A forward whose seq_lens or q_start hold other lengths than the plan was built from
+ * stays inside its buffers, but its result may be wrong: it then records code 8. */
 PA_API int pa_paged_plan(const pa_paged_attn_args* args, void* plan, size_t plan_bytes,
                          pa_stream_t stream);
 
@@ -407,8 +408,9 @@ PA_API int pa_paged_plan(const pa_paged_attn_args* args, void* plan, size_t plan
 PA_API int pa_paged_attn(const pa_paged_attn_args* args, void* plan, size_t plan_bytes,
                          void* scratch, size_t scratch_bytes, pa_stream_t stream);
 
-/* Status of the forwards on `plan` since it was built, synchronising `stream`: 0, or the
- * device code of a bounded wait that ran out (PA_ERR_DEVICE). */
+/* Status of the forwards on `plan` since it was built, synchronising `stream`: 0, or a device
+ * code and PA_ERR_DEVICE: 8 = the plan was built from other lengths than a forward's, else
+ * the code of a bounded wait that ran out (as pa_attn_status). */
 PA_API int pa_paged_status(const void* plan, int32_t* status_host, pa_stream_t stream);
 
 #ifdef __cplusplus

@@ -12,6 +12,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "libpolyattn_sm100.so"
 
 PA_OK, PA_ERR_ARG, PA_ERR_CUDA, PA_ERR_UNSUPPORTED, PA_ERR_DEVICE = 0, -1, -2, -3, -4
+DEV_OTHER_LENGTHS = 8    # device code: a paged plan was built from other lengths
 PA_BF16, PA_F16 = 0, 1
 
 c_i32, c_i64, c_f32, c_vp, c_sz = (ctypes.c_int32, ctypes.c_int64, ctypes.c_float,

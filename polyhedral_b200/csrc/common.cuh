@@ -22,6 +22,7 @@ enum : int32_t {
   DEV_TIMEOUT_O = 5,        // epilogue waited too long for O
   DEV_TIMEOUT_DRAIN = 6,    // teardown could not drain outstanding copies
   DEV_TIMEOUT_ITEM = 7,     // a wait on the work-item ring ran out
+  DEV_OTHER_LENGTHS = 8,    // a paged plan was built from other lengths than the call's
 };
 
 // A wait gives up after this many nanoseconds of %globaltimer.  One kernel step

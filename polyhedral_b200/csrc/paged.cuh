@@ -152,6 +152,26 @@ struct __align__(16) Cut {
   Request R;
 };
 
+// Whether the plan was built from other lengths than the arrays hold now, as far as shares
+// w0, w0 + step, ... and requests in the same steps can tell.  A worker takes the request that
+// its share begins in from the plan and all others from the arrays, so a result can only be
+// wrong where such a request has changed, or where one has rows now that lies before the
+// first share (or any, if the plan has no share).
+__device__ __forceinline__ bool other_lengths(const Params& P, const Share* shares, int used, int w0,
+                                              int step) {
+  bool other = false;
+  for (int w = w0; w < used; w += step) {
+    const Share s = shares[w];
+    if (s.b >= P.requests) break;
+    const Request R = get_request(P, s.b);
+    other |= R.row0 != s.R.row0 || R.n != s.R.n || R.pos0 != s.R.pos0 ||
+             R.len != min(s.R.len, P.width << P.page_shift);
+  }
+  const int idle = used > 0 ? min(shares[0].b, P.requests) : P.requests;
+  for (int b = w0; b < idle; b += step) other |= get_request(P, b).n > 0;
+  return other;
+}
+
 // What the host chooses from the sizes and hints alone, alike for plan and forward.
 struct Config {
   int unit_rows;      // query rows per unit
@@ -169,7 +189,7 @@ constexpr int kUnitCost = 2;
 struct PlanView {
   int32_t* status;
   int32_t* meta;      // shares in use, divided units, most rows of a unit
-  Share* shares;      // [workers + 1]
+  Share* shares;      // [workers + 1]; the entry behind those in use is past all requests
   Cut* cuts;          // [workers] divided units
   long long* before;  // [requests + 1] cost before a request
 };

@@ -188,6 +188,7 @@ int launch_chunk(const pa_paged_attn_args* a, const Params& P, const Config& c, 
   if ((rc = make_map(&tv, a->v_cache, a->dtype, a->D, {a->page_size, a->kv_heads, a->pages},
                      {a->v_row_stride, a->v_head_stride, a->v_page_stride}, C.seg, 1, "v_cache")))
     return rc;
+  C.check = !c.split;
   C.o32 = aligned(a->o, 32) && a->o_token_stride % 16 == 0 && a->o_head_stride % 16 == 0;
   const uint32_t fmt = a->dtype == PA_BF16 ? 1u : 0u;
   C.idesc_qk = make_idesc_f16(fmt, 128, 128, 0, 0);

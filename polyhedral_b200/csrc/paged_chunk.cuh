@@ -53,6 +53,7 @@ struct ChunkParams {
   int tb;                 // tokens per half: 128 / group
   int seg, nseg;          // rows of a page's box, boxes per super-tile
   int o32;                // rows of o are 32-byte aligned
+  int check;              // compare the plan's lengths
   uint32_t idesc_qk, idesc_pv;
   ErrSink err;
 };
@@ -231,7 +232,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   };
   pdl_wait();
   pdl_begin_next();
-  if ((int)blockIdx.x >= __ldg(meta)) return;   // no share: the whole CTA leaves
+  // no share: the whole CTA leaves, but for the first, which may have lengths to compare
+  if ((int)blockIdx.x >= max(__ldg(meta), 1)) return;
 
   if (threadIdx.x == 0) {
     for (int h = 0; h < 2; ++h) {
@@ -400,6 +402,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           }
           page = next;
         }
+      }
+      // the plan's lengths, where no join compares them, while the last copies are on their way
+      // and used (in a warp of its own, or before the warps part, this made the D = 64 softmax
+      // spill 44-96 bytes)
+      if (C.check) {
+        const int used = __ldg(meta);            // CTAs that are here: these, or the first alone
+        if (other_lengths(P, shares, used, w * 32 + lane, max(used, 1) * 32))
+          err.record(DEV_OTHER_LENGTHS);
       }
       // every copy issued lands before the CTA can exit
       if (lane == 0) {

@@ -107,7 +107,7 @@ __device__ __noinline__ void piece_by_key(const Params& P, const Piece& c) {
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kFewWarps * 32, 1)
 paged_few_kernel(const __grid_constant__ Params P, const Share* __restrict__ shares,
-                 const int32_t* __restrict__ meta, float* __restrict__ scratch) {
+                 const int32_t* __restrict__ meta, float* __restrict__ scratch, int32_t* status) {
   using F = Few<D>;
   constexpr int S = F::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -120,6 +120,11 @@ paged_few_kernel(const __grid_constant__ Params P, const Share* __restrict__ sha
   uint32_t* s_live = reinterpret_cast<uint32_t*>(smem + F::kMetaOff) + warp * S;
   const int used = __ldg(meta);
   const Share first = shares[w], end = shares[w + 1];   // inside the plan for every worker
+  // the plan's lengths, where no join compares them: by the last workers, which have no share
+  // where the work is little
+  if (status && warp == kFewWarps - 1 &&
+      other_lengths(P, shares, used, (gridDim.x - 1 - blockIdx.x) * 32 + lane, gridDim.x * 32))
+    atomicExch(status, (int32_t)DEV_OTHER_LENGTHS);
   if (w >= used) return;
   const int G = P.group;
   const int mask = (1 << P.page_shift) - 1;
@@ -403,22 +408,23 @@ paged_few_kernel(const __grid_constant__ Params P, const Share* __restrict__ sha
 
 namespace {
 template <int D, bool kBf16>
-int launch_few_body(const Params& P, const PlanView& pv, float* scratch, int sms,
+int launch_few_body(const Params& P, const PlanView& pv, const Config& c, float* scratch, int sms,
                     cudaStream_t stream) {
   const int rc = prepare_kernel<paged_few_kernel<D, kBf16>>(Few<D>::kBytes, 0);
   if (rc) return rc;
   return launch_after("pa_paged_attn", paged_few_kernel<D, kBf16>, sms, kFewWarps * 32, Few<D>::kBytes,
-                      stream, P, pv.shares, pv.meta, scratch);
+                      stream, P, pv.shares, pv.meta, scratch,
+                      c.split ? nullptr : pv.status);
 }
 }  // namespace
 
 int launch_few(const Params& P, bool bf16, int D, const PlanView& pv, const Config& c,
                float* scratch, int sms, cudaStream_t stream) {
   if (D == 128)
-    return bf16 ? launch_few_body<128, true>(P, pv, scratch, sms, stream)
-                : launch_few_body<128, false>(P, pv, scratch, sms, stream);
-  return bf16 ? launch_few_body<64, true>(P, pv, scratch, sms, stream)
-              : launch_few_body<64, false>(P, pv, scratch, sms, stream);
+    return bf16 ? launch_few_body<128, true>(P, pv, c, scratch, sms, stream)
+                : launch_few_body<128, false>(P, pv, c, scratch, sms, stream);
+  return bf16 ? launch_few_body<64, true>(P, pv, c, scratch, sms, stream)
+              : launch_few_body<64, false>(P, pv, c, scratch, sms, stream);
 }
 
 }  // namespace paged

@@ -239,6 +239,7 @@ paged_plan_kernel(const __grid_constant__ Params P, Config c, PlanView pv) {
   }
   __syncthreads();
   if (threadIdx.x == 0) {
+    if (used == 0) pv.shares[0] = Share{B, 0, 0, 0, {0, 0, 0, 0}};
     pv.meta[0] = used;
     pv.meta[1] = s_cuts;
     pv.meta[2] = s_rows;
@@ -267,6 +268,12 @@ paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
   pdl_wait();
   pdl_begin_next();
   const int used = pv.meta[0], cuts = pv.meta[1], rows = pv.meta[2];
+  // the plan's lengths, by the last CTAs, which have no row where the work is little
+  {
+    const int x = (gridDim.x - 1 - blockIdx.x) * (kJoinWarps * 32) + threadIdx.x;
+    if (other_lengths(P, pv.shares, used, x, gridDim.x * kJoinWarps * 32))
+      atomicExch(pv.status, (int32_t)DEV_OTHER_LENGTHS);
+  }
   const bool many = used > kJoinWarps * cuts;   // pieces per unit, on average
   const int unit_rows = c.unit_rows;
   const size_t slot = slot_floats<D>(unit_rows);

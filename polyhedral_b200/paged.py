@@ -199,9 +199,10 @@ def _plan_sizes(head, device):
 
 
 class PagedPlan:
-    """Shares of work of one step's attention (``make_plan``): the same for every layer,
-    read by the forwards and never written, so they may run on several streams.  It
-    keeps the ``seq_lens`` and ``q_start`` it was built from."""
+    """Shares of work of one step's attention (``make_plan``): the same for every layer, and
+    only read by the forwards (but for a status word, which a failure sets), so they may run on
+    several streams.  It keeps the ``seq_lens`` and ``q_start`` it was built from; a forward
+    that is given other lengths reports it (``status``)."""
 
     __slots__ = ("buffer", "nbytes", "scratch_bytes", "key", "head", "tail", "device",
                  "seq_lens", "q_start")
@@ -216,8 +217,9 @@ class PagedPlan:
                 self.buffer.data_ptr(), self.nbytes)
 
     def status(self):
-        """Device status of the forwards on this plan so far (synchronises): 0, or the code
-        of the bounded wait that ran out."""
+        """Device status of the forwards on this plan so far (synchronises): 0,
+        ``_lib.DEV_OTHER_LENGTHS`` where one was given other lengths than the plan was built
+        from, or the code of a bounded wait that ran out."""
         return _lib.device_status("pa_paged_status", self.buffer)
 
 
@@ -260,8 +262,10 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, q_start, kind, p
     hold no keys.
 
     ``plan`` is ``make_plan``'s for these lengths and this mask; without one it is built
-    first (``max_new`` / ``max_len`` as there).  ``out`` / ``lse_out`` are written in place of
-    new tensors.  ``check`` synchronises and raises if the kernel reported a failure."""
+    first (``max_new`` / ``max_len`` as there).  The plan of another step gives wrong results
+    and is reported: ``check`` or ``plan.status()`` shows it.  ``out`` / ``lse_out`` are written
+    in place of new tensors.  ``check`` synchronises and raises if the kernel reported a
+    failure."""
     if q.dim() != 3:
         raise ValueError("q must be [tokens, heads, D]")
     (pages, page_size, Hkv, Dc), ks, vs = _caches(k_cache, v_cache)
@@ -325,5 +329,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, q_start, kind, p
         st = plan.status()
         if st:
             raise _lib.PolyattnError("pa_paged_attn", _lib.PA_ERR_DEVICE,
-                                     f"device status {st} (a bounded wait ran out)")
+                                     f"device status {st} (" +
+                                     ("the plan was built from other lengths"
+                                      if st == _lib.DEV_OTHER_LENGTHS else
+                                      "a bounded wait ran out") + ")")
     return (o, lse) if return_lse else o
