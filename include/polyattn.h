@@ -413,6 +413,16 @@ PA_API int pa_paged_attn(const pa_paged_attn_args* args, void* plan, size_t plan
  * the code of a bounded wait that ran out (as pa_attn_status). */
 PA_API int pa_paged_status(const void* plan, int32_t* status_host, pa_stream_t stream);
 
+/* Test hook for the failure path: pa_paged_attn with every bounded wait of the chunk kernel
+ * limited to wait_limit_ns (1 us .. 1 s; the waits for Q tiles to a quarter of it, so they run
+ * out first) and the Q tiles of each unit's first half never loaded.  The kernel records code
+ * 1, stops, drains its copies and products, frees TMEM and ends; pa_paged_status reports it.
+ * Outputs are unspecified.  Sizes that run the few-rows kernel, which waits for no barrier,
+ * are refused with PA_ERR_UNSUPPORTED. */
+PA_API int pa_paged_attn_withheld(const pa_paged_attn_args* args, void* plan, size_t plan_bytes,
+                                  void* scratch, size_t scratch_bytes, int64_t wait_limit_ns,
+                                  pa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -128,6 +128,7 @@ SIGNATURES = {
     "pa_paged_scratch_size": (c_sz, [c_vp]),
     "pa_paged_plan": (ctypes.c_int, [c_vp, c_vp, c_sz, c_vp]),
     "pa_paged_attn": (ctypes.c_int, [c_vp, c_vp, c_sz, c_vp, c_sz, c_vp]),
+    "pa_paged_attn_withheld": (ctypes.c_int, [c_vp, c_vp, c_sz, c_vp, c_sz, c_i64, c_vp]),
     "pa_paged_status": (ctypes.c_int, [c_vp, ctypes.POINTER(c_i32), c_vp]),
     "pa_paged_append": (ctypes.c_int, [c_vp, c_vp]),
 }

@@ -170,7 +170,7 @@ int make_map(CUtensorMap* m, const void* base, int dtype, int D, const long long
 }
 
 int launch_chunk(const pa_paged_attn_args* a, const Params& P, const Config& c, const PlanView& pv,
-                 float* scratch, int sms, cudaStream_t stream) {
+                 float* scratch, int sms, cudaStream_t stream, uint64_t wait_ns, int withhold_q) {
   CUtensorMap tq, tk, tv;
   int rc;
   ChunkParams C;
@@ -195,7 +195,9 @@ int launch_chunk(const pa_paged_attn_args* a, const Params& P, const Config& c, 
   C.idesc_pv = make_idesc_f16(fmt, 128, a->D, 0, 1);
   C.err.word = pv.status;
   C.err.epoch = 0;
-  C.err.limit_ns = kWaitLimitNs;
+  C.err.limit_ns = wait_ns;
+  C.q_limit_ns = withhold_q ? wait_ns / 4 : wait_ns;
+  C.withhold_q = withhold_q;
   return a->D == 128 ? launch_chunk_d128(tq, tk, tv, C, fmt != 0, pv, scratch, sms, stream)
                      : launch_chunk_d64(tq, tk, tv, C, fmt != 0, pv, scratch, sms, stream);
 }
@@ -204,6 +206,35 @@ size_t scratch_bytes_of(const pa_paged_attn_args* a, const Config& c) {
   if (!c.split) return 0;
   const size_t f = a->D == 128 ? slot_floats<128>(c.unit_rows) : slot_floats<64>(c.unit_rows);
   return 2 * (size_t)c.workers * f * sizeof(float);
+}
+
+// The forward, with the limit of its bounded waits; withhold_q: pa_paged_attn_withheld.
+int forward(const pa_paged_attn_args* a, void* plan, size_t plan_size, void* scratch,
+            size_t scratch_bytes, cudaStream_t stream, uint64_t wait_ns, int withhold_q,
+            const char* who) {
+  int rc = check_sizes(a, who), sms = 0;
+  if (rc) return rc;
+  if (a->tokens == 0) return PA_OK;
+  if ((rc = check_args(a, who))) return rc;
+  Params P;
+  if ((rc = make_params(a, &P, who))) return rc;
+  if ((rc = sm_count(&sms))) return rc;
+  const Config c = choose(a, sms);
+  PA_CHECK_ARG(plan && plan_size >= plan_bytes(c, a->requests) && aligned(plan, 256),
+               "%s: plan must be 256-byte aligned and >= %zu bytes", who, plan_bytes(c, a->requests));
+  const size_t need = scratch_bytes_of(a, c);
+  PA_CHECK_ARG(need == 0 || (scratch && scratch_bytes >= need && aligned(scratch, 256)),
+               "%s: scratch must be 256-byte aligned and >= %zu bytes", who, need);
+  if (withhold_q && !c.half_tokens)
+    return fail(PA_ERR_UNSUPPORTED, "%s: these sizes run the few-rows kernel, which waits for no barrier",
+                who);
+  const PlanView pv = plan_view(plan, c);
+  const bool bf = a->dtype == PA_BF16;
+  float* part = static_cast<float*>(scratch);
+  rc = c.half_tokens ? launch_chunk(a, P, c, pv, part, sms, stream, wait_ns, withhold_q)
+                     : launch_few(P, bf, a->D, pv, c, part, sms, stream);
+  if (rc) return rc;
+  return c.split ? launch_join(P, bf, a->D, pv, c, part, sms, stream) : PA_OK;
 }
 
 }  // namespace
@@ -245,30 +276,19 @@ extern "C" int pa_paged_plan(const pa_paged_attn_args* a, void* plan, size_t pla
 
 extern "C" int pa_paged_attn(const pa_paged_attn_args* a, void* plan, size_t plan_size,
                              void* scratch, size_t scratch_bytes, pa_stream_t stream) {
+  return pa::paged::forward(a, plan, plan_size, scratch, scratch_bytes, (cudaStream_t)stream,
+                            pa::kWaitLimitNs, 0, "pa_paged_attn");
+}
+
+extern "C" int pa_paged_attn_withheld(const pa_paged_attn_args* a, void* plan, size_t plan_size,
+                                      void* scratch, size_t scratch_bytes, int64_t wait_limit_ns,
+                                      pa_stream_t stream) {
   using namespace pa;
-  using namespace pa::paged;
-  int rc = check_sizes(a, "pa_paged_attn"), sms = 0;
-  if (rc) return rc;
-  if (a->tokens == 0) return PA_OK;
-  if ((rc = check_args(a, "pa_paged_attn"))) return rc;
-  Params P;
-  if ((rc = make_params(a, &P, "pa_paged_attn"))) return rc;
-  if ((rc = sm_count(&sms))) return rc;
-  const Config c = choose(a, sms);
-  PA_CHECK_ARG(plan && plan_size >= plan_bytes(c, a->requests) && aligned(plan, 256),
-               "pa_paged_attn: plan must be 256-byte aligned and >= %zu bytes",
-               plan_bytes(c, a->requests));
-  const size_t need = scratch_bytes_of(a, c);
-  PA_CHECK_ARG(need == 0 || (scratch && scratch_bytes >= need && aligned(scratch, 256)),
-               "pa_paged_attn: scratch must be 256-byte aligned and >= %zu bytes", need);
-  const PlanView pv = plan_view(plan, c);
-  const cudaStream_t s = (cudaStream_t)stream;
-  const bool bf = a->dtype == PA_BF16;
-  rc = c.half_tokens ? launch_chunk(a, P, c, pv, static_cast<float*>(scratch), sms, s)
-                     : launch_few(P, bf, a->D, pv, c, static_cast<float*>(scratch), sms, s);
-  if (rc) return rc;
-  return c.split ? launch_join(P, bf, a->D, pv, c, static_cast<const float*>(scratch), sms, s)
-                 : PA_OK;
+  PA_CHECK_ARG(wait_limit_ns >= 1000 && wait_limit_ns <= (int64_t)kWaitLimitNs,
+               "pa_paged_attn_withheld: wait_limit_ns=%lld outside [1 us, 1 s]",
+               (long long)wait_limit_ns);
+  return paged::forward(a, plan, plan_size, scratch, scratch_bytes, (cudaStream_t)stream,
+                        (uint64_t)wait_limit_ns, 1, "pa_paged_attn_withheld");
 }
 
 extern "C" int pa_paged_status(const void* plan, int32_t* status_host, pa_stream_t stream) {

@@ -55,7 +55,9 @@ struct ChunkParams {
   int o32;                // rows of o are 32-byte aligned
   int check;              // compare the plan's lengths
   uint32_t idesc_qk, idesc_pv;
-  ErrSink err;
+  int withhold_q;         // test hook: the Q tiles of half 0 are never loaded
+  uint64_t q_limit_ns;    // limit of the waits for Q tiles
+  ErrSink err;            // status word, limit of all other waits
 };
 
 // What decides, for one half of a unit, the kind of the super-tile at key kb: some row sees
@@ -213,13 +215,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const ErrSink& err = C.err;
   // A bounded wait (mbar_wait); the time in which a warp goes key by key does not count.
-  auto wait_bar = [&](uint64_t* bar, uint32_t parity, int32_t code) -> bool {
+  auto wait_for = [&](uint64_t* bar, uint32_t parity, int32_t code, uint64_t limit_ns) -> bool {
     if (mbar_try_wait(bar, parity)) return true;
     uint64_t t0 = globaltimer();
     while (true) {
       if (mbar_try_wait(bar, parity)) return true;
       if (*s_abort) return false;
-      if (globaltimer() - t0 > err.limit_ns) {
+      if (globaltimer() - t0 > limit_ns) {
         if (*static_cast<volatile int*>(s_slow) > 0) {
           t0 = globaltimer();
           continue;
@@ -229,6 +231,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         return false;
       }
     }
+  };
+  auto wait_bar = [&](uint64_t* bar, uint32_t parity, int32_t code) -> bool {
+    return wait_for(bar, parity, code, err.limit_ns);
   };
   pdl_wait();
   pdl_begin_next();
@@ -351,6 +356,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
               ok = 0;
               break;
             }
+            if (h == 0 && C.withhold_q) continue;
             mbar_arrive_expect_tx(&q_full[h], C.tb * P.group * D * 2);
             ++q_armed[h];
             for (int c = 0; c < kParts; ++c)
@@ -507,7 +513,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         if (tiles <= 0) continue;
         const int halves = n > C.tb ? 2 : 1;
         for (int h = 0; h < halves && ok; ++h) {
-          ok = wait_all(&q_full[h], tq[h] & 1, DEV_TIMEOUT_Q);
+          ok = __all_sync(0xffffffffu, wait_for(&q_full[h], tq[h] & 1, DEV_TIMEOUT_Q, C.q_limit_ns));
+          tc_fence_after();
           ++tq[h];
         }
         uint32_t ks = 0, vs = 0;
