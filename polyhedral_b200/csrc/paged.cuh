@@ -111,24 +111,24 @@ __device__ __forceinline__ KeyRanges key_ranges(const Pred& p, int i0, int i1, i
   return r;
 }
 
-// Allows kernel kKernel `smem` bytes of shared memory, once per device; with `min_regs`,
-// refuses a build with fewer registers per thread (a register split that they do not cover
-// would never complete).
+// Allows kernel kKernel `smem` bytes of shared memory, once per device and always the same
+// (the limit belongs to the function: a smaller one set by another thread's call would make a
+// launch fail); with `min_regs`, refuses a build with fewer registers per thread (a register
+// split that they do not cover would never complete).
 template <auto kKernel>
-int prepare_kernel(int smem, int min_regs) {
+int prepare_kernel(const char* who, int smem, int min_regs) {
   static std::atomic<uint64_t> done{0};
   int dev = 0;
-  PA_CUDA(cudaGetDevice(&dev), "pa_paged_attn");
+  PA_CUDA(cudaGetDevice(&dev), who);
   const uint64_t bit = 1ull << (dev & 63);
   if (done.load(std::memory_order_relaxed) & bit) return PA_OK;
-  PA_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-          "pa_paged_attn");
+  PA_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), who);
   if (min_regs > 0) {
     cudaFuncAttributes fa;
-    PA_CUDA(cudaFuncGetAttributes(&fa, kKernel), "pa_paged_attn");
+    PA_CUDA(cudaFuncGetAttributes(&fa, kKernel), who);
     if (fa.numRegs < min_regs)
-      return fail(PA_ERR_UNSUPPORTED, "pa_paged_attn: kernel built with %d registers per thread, "
-                  "below its register split", fa.numRegs);
+      return fail(PA_ERR_UNSUPPORTED, "%s: kernel built with %d registers per thread, below its "
+                  "register split", who, fa.numRegs);
   }
   done.fetch_or(bit, std::memory_order_relaxed);
   return PA_OK;

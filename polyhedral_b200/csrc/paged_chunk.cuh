@@ -896,7 +896,8 @@ int launch_chunk_body(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
                       const ChunkParams& C, const PlanView& pv, float* scratch, int sms,
                       cudaStream_t stream) {
   constexpr int kMinRegs = (256 * kChunkSoftRegs + 128 * kChunkOtherRegs) / kChunkThreads;
-  const int rc = prepare_kernel<paged_chunk_kernel<D, kBf16>>(ChunkSmem<D>::kAlloc, kMinRegs);
+  const int rc = prepare_kernel<paged_chunk_kernel<D, kBf16>>("pa_paged_attn", ChunkSmem<D>::kAlloc,
+                                                              kMinRegs);
   if (rc) return rc;
   return launch_after("pa_paged_attn", paged_chunk_kernel<D, kBf16>, sms, kChunkThreads,
                       ChunkSmem<D>::kAlloc, stream, tq, tk, tv, C, pv.shares, pv.meta, scratch);

@@ -410,7 +410,7 @@ namespace {
 template <int D, bool kBf16>
 int launch_few_body(const Params& P, const PlanView& pv, const Config& c, float* scratch, int sms,
                     cudaStream_t stream) {
-  const int rc = prepare_kernel<paged_few_kernel<D, kBf16>>(Few<D>::kBytes, 0);
+  const int rc = prepare_kernel<paged_few_kernel<D, kBf16>>("pa_paged_attn", Few<D>::kBytes, 0);
   if (rc) return rc;
   return launch_after("pa_paged_attn", paged_few_kernel<D, kBf16>, sms, kFewWarps * 32, Few<D>::kBytes,
                       stream, P, pv.shares, pv.meta, scratch,

@@ -13,8 +13,7 @@
 // rather than read a table entry that another CTA writes.  3.4 us on the GPU for 8 requests
 // of one token, launch included, in a captured graph; 1000 requests with 65313 tokens take
 // 13.5 us a call, which is the host's side of it.
-#include "common.cuh"
-#include "capi_util.h"
+#include "paged.cuh"
 
 namespace pa {
 namespace {
@@ -226,9 +225,11 @@ extern "C" int pa_paged_step(const pa_paged_step_args* a, pa_stream_t stream) {
       PA_CHECK_ARG(x.n == 0 || y.n == 0 || x.p + x.n <= y.p || y.p + y.n <= x.p,
                    "pa_paged_step: an output overlaps old_lens, new_lens, free_pages or free_head");
   const int smem = (a->requests + 1) * (int)sizeof(int2);
-  if (smem > 40 * 1024)
-    PA_CUDA(cudaFuncSetAttribute(paged_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 smem), "pa_paged_step");
+  if (smem > 40 * 1024) {
+    const int rc = paged::prepare_kernel<paged_step_kernel>(
+        "pa_paged_step", (kMaxRequests + 1) * (int)sizeof(int2), 0);
+    if (rc) return rc;
+  }
   int grid = (a->tokens + kStepThreads - 1) / kStepThreads;
   grid = grid < 1 ? 1 : grid > 148 ? 148 : grid;
   return launch_after("pa_paged_step", paged_step_kernel, grid, kStepThreads, smem,
