@@ -309,8 +309,9 @@ PA_API int pa_lse_merge(const pa_merge_args* args, pa_stream_t stream);
  *     *missing = pages that could not be had, because the free list ran out or the
  *     table is too narrow: their table entries (inside the table) and their tokens'
  *     slots are -1.
- * Negative lengths count as 0; new tokens in all stay below 2^31.  No output may overlap
- * old_lens, new_lens, free_pages or free_head. */
+ * Negative lengths count as 0; new tokens in all stay below 2^31.  A request's tokens behind
+ * its 2^31-th have no position: slot and position -1, and its length stays at 2^31 - 1.  No
+ * output may overlap old_lens, new_lens, free_pages or free_head. */
 typedef struct pa_paged_step_args {
   int32_t requests;            /* 1 .. 16384 */
   int32_t page_size;           /* >= 1 */

@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(pa_paged_step_
       const long long have = div_up(c), need = div_up((long long)c + n);
       np = (int)(max(min(need, W), min(have, W)) - min(have, W));
       over += (int)(need - have) - np;
-      if (blockIdx.x == 0) a.seq_lens[b] = c + n;
+      if (blockIdx.x == 0) a.seq_lens[b] = (int)min((long long)c + n, 0x7fffffffll);
     }
     int st = n, sp = np, tt, tp;
     block_scan2(st, sp, tt, tp, warp_sum);
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(pa_paged_step_
   }
   if (threadIdx.x == 0) pre[B] = make_int2(base_t, base_p);
   const int head = min(max(__ldg(a.free_head), 0), a.free_count);
-  const int got = min(base_p, a.free_count - head);
+  const int got = max(min(base_p, a.free_count - head), 0);
   if (blockIdx.x == 0) {
     const int left_out = __syncthreads_or(over != 0);
     __shared__ int sum_over;
@@ -113,6 +113,8 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(pa_paged_step_
 
   const int tid = blockIdx.x * kStepThreads + threadIdx.x;
   const int step = gridDim.x * kStepThreads;
+  // Columns are compared with the table's width, and entries of the free list with those to
+  // be had, also where sums of absurd lengths have overflowed: nothing outside is touched.
   // page id for a slot, or -1 when the slot would not fit in 32 bits (no such page)
   auto page_ok = [P](int page) { return page >= 0 && (long long)(page + 1ll) * P <= 0x7fffffffll; };
   for (int t = tid; t < a.tokens; t += step) {
@@ -120,19 +122,22 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(pa_paged_step_
     if (t < base_t) {
       const int b = find_request(pre, B, t, false);
       const int c = max(__ldg(a.old_lens + b), 0);
-      pos = c + (t - pre[b].x);
-      const long long have = div_up(c);
-      const int col = pos / P;
-      int page = -1;
-      if (col < W) {
-        if (col < have) {
-          page = a.block_table[b * a.table_stride + col];   // not written by this launch
-        } else {
-          const int x = pre[b].y + (int)(col - have);
-          if (x < got) page = __ldg(a.free_pages + head + x);
+      const long long at = (long long)c + t - pre[b].x;
+      if (at >= 0 && at <= 0x7fffffffll) {
+        pos = (int)at;
+        const long long have = div_up(c);
+        const int col = pos / P;
+        int page = -1;
+        if (col < W) {
+          if (col < have) {
+            page = a.block_table[b * a.table_stride + col];   // not written by this launch
+          } else {
+            const long long x = pre[b].y + (col - have);
+            if (x >= 0 && x < got) page = __ldg(a.free_pages + head + x);
+          }
         }
+        if (page_ok(page)) slot = page * P + (pos - col * P);
       }
-      if (page_ok(page)) slot = page * P + (pos - col * P);
     }
     a.slot_map[t] = slot;
     a.positions[t] = pos;
@@ -140,7 +145,8 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(pa_paged_step_
   for (int x = tid; x < base_p; x += step) {
     const int b = find_request(pre, B, x, true);
     const long long col = div_up(max(__ldg(a.old_lens + b), 0)) + (x - pre[b].y);
-    a.block_table[b * a.table_stride + col] = x < got ? __ldg(a.free_pages + head + x) : -1;
+    if (col >= 0 && col < W)
+      a.block_table[b * a.table_stride + col] = x < got ? __ldg(a.free_pages + head + x) : -1;
   }
 }
 
