@@ -111,6 +111,14 @@ __device__ __forceinline__ KeyRanges key_ranges(const Pred& p, int i0, int i1, i
   return r;
 }
 
+// Multiprocessors of the current device.
+inline int sm_count(int* sms, const char* who) {
+  int dev = 0;
+  PA_CUDA(cudaGetDevice(&dev), who);
+  PA_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev), who);
+  return PA_OK;
+}
+
 // Allows kernel kKernel `smem` bytes of shared memory, once per device and always the same
 // (the limit belongs to the function: a smaller one set by another thread's call would make a
 // launch fail); with `min_regs`, refuses a build with fewer registers per thread (a register

@@ -88,13 +88,6 @@ int make_params(const pa_paged_attn_args* a, Params* P, const char* who) {
   return make_pred(&pr, &P->pred, who);
 }
 
-int sm_count(int* sms) {
-  int dev = 0;
-  PA_CUDA(cudaGetDevice(&dev), "pa_paged_attn");
-  PA_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev), "pa_paged_attn");
-  return PA_OK;
-}
-
 // Kernel and shares for these sizes and hints.
 Config choose(const pa_paged_attn_args* a, int sms) {
   Config c;
@@ -221,7 +214,7 @@ int forward(const pa_paged_attn_args* a, void* plan, size_t plan_size, void* scr
   if ((rc = check_args(a, who))) return rc;
   Params P;
   if ((rc = make_params(a, &P, who))) return rc;
-  if ((rc = sm_count(&sms))) return rc;
+  if ((rc = sm_count(&sms, who))) return rc;
   const Config c = choose(a, sms);
   PA_CHECK_ARG(plan && plan_size >= plan_bytes(c, a->requests) && aligned(plan, 256),
                "%s: plan must be 256-byte aligned and >= %zu bytes", who, plan_bytes(c, a->requests));
@@ -247,14 +240,14 @@ int forward(const pa_paged_attn_args* a, void* plan, size_t plan_size, void* scr
 extern "C" size_t pa_paged_plan_size(const pa_paged_attn_args* a) {
   using namespace pa::paged;
   int sms = 0;
-  if (check_sizes(a, "pa_paged_plan_size") || sm_count(&sms)) return 0;
+  if (check_sizes(a, "pa_paged_plan_size") || sm_count(&sms, "pa_paged_plan_size")) return 0;
   return plan_bytes(choose(a, sms), a->requests);
 }
 
 extern "C" size_t pa_paged_scratch_size(const pa_paged_attn_args* a) {
   using namespace pa::paged;
   int sms = 0;
-  if (check_sizes(a, "pa_paged_scratch_size") || sm_count(&sms)) return 0;
+  if (check_sizes(a, "pa_paged_scratch_size") || sm_count(&sms, "pa_paged_scratch_size")) return 0;
   return scratch_bytes_of(a, choose(a, sms));
 }
 
@@ -269,7 +262,7 @@ extern "C" int pa_paged_plan(const pa_paged_attn_args* a, void* plan, size_t pla
                a->table_width, a->page_size);
   Params P;
   if ((rc = make_params(a, &P, "pa_paged_plan"))) return rc;
-  if ((rc = sm_count(&sms))) return rc;
+  if ((rc = sm_count(&sms, "pa_paged_plan"))) return rc;
   const Config c = choose(a, sms);
   PA_CHECK_ARG(plan && plan_size >= plan_bytes(c, a->requests) && aligned(plan, 256),
                "pa_paged_plan: plan must be 256-byte aligned and >= %zu bytes",

@@ -236,8 +236,11 @@ extern "C" int pa_paged_step(const pa_paged_step_args* a, pa_stream_t stream) {
         "pa_paged_step", (kMaxRequests + 1) * (int)sizeof(int2), 0);
     if (rc) return rc;
   }
-  int grid = (a->tokens + kStepThreads - 1) / kStepThreads;
-  grid = grid < 1 ? 1 : grid > 148 ? 148 : grid;
+  int sms = 0;
+  const int rc = paged::sm_count(&sms, "pa_paged_step");
+  if (rc) return rc;
+  int grid = a->tokens / kStepThreads + (a->tokens % kStepThreads != 0);
+  grid = grid < 1 ? 1 : grid > sms ? sms : grid;
   return launch_after("pa_paged_step", paged_step_kernel, grid, kStepThreads, smem,
                       (cudaStream_t)stream, *a);
 }
