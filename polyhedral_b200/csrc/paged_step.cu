@@ -112,12 +112,13 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(pa_paged_step_
   __syncthreads();
 
   const int tid = blockIdx.x * kStepThreads + threadIdx.x;
-  const int step = gridDim.x * kStepThreads;
+  const int step = gridDim.x * kStepThreads;   // steps in 64 bits: the last one may pass 2^31
   // Columns are compared with the table's width, and entries of the free list with those to
   // be had, also where sums of absurd lengths have overflowed: nothing outside is touched.
   // page id for a slot, or -1 when the slot would not fit in 32 bits (no such page)
   auto page_ok = [P](int page) { return page >= 0 && (long long)(page + 1ll) * P <= 0x7fffffffll; };
-  for (int t = tid; t < a.tokens; t += step) {
+  for (long long i = tid; i < a.tokens; i += step) {
+    const int t = (int)i;
     int slot = -1, pos = -1;
     if (t < base_t) {
       const int b = find_request(pre, B, t, false);
@@ -142,7 +143,8 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(pa_paged_step_
     a.slot_map[t] = slot;
     a.positions[t] = pos;
   }
-  for (int x = tid; x < base_p; x += step) {
+  for (long long i = tid; i < base_p; i += step) {
+    const int x = (int)i;
     const int b = find_request(pre, B, x, true);
     const long long col = div_up(max(__ldg(a.old_lens + b), 0)) + (x - pre[b].y);
     if (col >= 0 && col < W)
@@ -272,7 +274,7 @@ extern "C" int pa_paged_append(const pa_paged_append_args* a, pa_stream_t stream
   const int vecs = a->kv_heads * a->D / 8;              // 16-byte vectors of a token
   const int tpc = vecs >= kAppendThreads ? 1 : kAppendThreads / vecs;
   const int per = tpc * kAppendRows;
-  const int grid = (a->tokens + per - 1) / per;
+  const int grid = a->tokens / per + (a->tokens % per != 0);
   return launch_after("pa_paged_append", paged_append_kernel, grid, kAppendThreads, 0,
                       (cudaStream_t)stream, *a, vecs, tpc);
 }

@@ -46,3 +46,21 @@ def test_tokens_behind_the_last_position(P, old, new):
     assert st.slot_map.tolist() == [-1 if g else s for g, s in zip(gone, ref[3])]
     assert st.positions.tolist() == [-1 if g else p for g, p in zip(gone, ref[4])]
     assert st.free_head.tolist() == [ref[5]] and st.missing.tolist() == [ref[6]]
+
+
+def test_slot_map_of_all_32_bits():
+    """2^31 - 1 entries, of which six tokens fill the first."""
+    from polyhedral_b200 import paged
+    T = TOP
+    table = torch.full((2, 3), -1, dtype=torch.int32, device="cuda")
+    guard = torch.full((3, 1000), 77, dtype=torch.int32, device="cuda")
+    st = paged.make_step(table, _i32([0, 15]), _i32([2, 4]), _i32([4, 9, 2]), _i32([0]), page_size=16,
+                         tokens=T)
+    assert st.slot_map[:6].tolist() == [64, 65, -1, 144, 145, 146]
+    assert st.positions[:6].tolist() == [0, 1, 15, 16, 17, 18]
+    for t in (st.slot_map, st.positions):
+        for part in t[6:].split(2**28):
+            assert bool((part == -1).all())
+    assert st.q_start.tolist() == [0, 2, 6] and st.seq_lens.tolist() == [2, 19]
+    assert st.free_head.tolist() == [2] and st.missing.tolist() == [0]
+    assert (guard == 77).all()
