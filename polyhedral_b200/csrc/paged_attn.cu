@@ -119,8 +119,12 @@ Config choose(const pa_paged_attn_args* a, int sms) {
     // anywhere, 24 us with pieces of 3; 22 requests of 356, 39 and 31 us
     c.min_piece = 3;
   }
-  // Requests of at most 128 tokens stay whole, which spares the join: 8 requests of some 100
-  // tokens, 14.1 us a call instead of 18.0 us (on the GPU alone 14.3 us instead of 13.3 us).
+  // Requests of at most 128 tokens stay whole, which spares the join's launch: 14.1 us a call
+  // instead of 18.2-18.5 us wherever the host bounds it.  On the GPU alone (captured) chunks gain
+  // too: 5 of 32 new tokens 7.1 us instead of 9.7, 8 of 60-100 16.5 instead of 18.0, 64 of them
+  // 48.4 instead of 52.1; decode by how many warps it fills: 500 of 20-126 tokens 42.2 instead of
+  // 42.8, 64 of 60-120 11.5 instead of 11.4, 8 of 100-120 10.6 instead of 9.3, one of 120 10.3
+  // instead of 8.1.
   c.split = !(a->max_len > 0 && a->max_len <= 128);
   return c;
 }

@@ -26,15 +26,18 @@
 // What bounds it: a half's chain per super-tile -- S read (100 cycles), its maximum (330),
 // the exponentials and P (1400; 1024 are the exponential unit's alone), then P V of the
 // second part and the next S (768 and the hand-overs) -- of which half runs under the other
-// half's products.  4096 new tokens over 16384, 32 heads of 128 sharing 8 key heads: 1076-1110
-// us = 1.12-1.15 PFLOP/s (of 1.64 measured for a library product in a burst, 1.40 sustained:
-// like that one it runs into the power limit, at 1.55 GHz); tensor cores and exponential
-// unit both 64 % busy.  8 chunks of 2000 under a window of 1024 and 4 sinks, a key head per
-// query head: 495 us = 0.54 PFLOP/s of live products; a unit has 11 super-tiles, 4 of a
-// half's 10 are partly masked and its first and last are the other half's, and between
-// units nothing overlaps a half's last products, result and first scores (7 000 of its
-// 45 000 cycles).  24 ragged requests, D = 64: 96 us = 0.48 PFLOP/s; there the exponentials of
-// both halves together are the limit.
+// half's products.  4096 new tokens over 16384, 32 heads of 128 sharing 8 key heads: 1010-1060
+// us in a short run, 1090-1140 in a long one = 1.09-1.22 PFLOP/s (of 1.64 measured for a
+// library product in a burst, 1.40 sustained: like that one it runs into the power limit, at
+// 1.55 GHz); tensor cores and exponential unit both 64 % busy.  8 chunks of 2000 under a window
+// of 1024 and 4 sinks, a key head per query head: 450-496 us = 0.54-0.60 PFLOP/s of live products;
+// a unit has 11 super-tiles, one of them for the 4 sinks, 4 of a half's 10 are partly masked
+// and its first and last are the other half's, and between units nothing overlaps a half's
+// last products, result and first scores (7 000 of its 45 000 cycles).  D = 64: no unit is
+// saturated.  The same chain with half the products leaves 4096 over 16384 at 780 us = 0.79
+// PFLOP/s (exponential unit 52 %, issue 53 %, tensor cores 35 % busy), and unit ends take their
+// share where units are short: 8 chunks of 1000 over 2000 0.64 PFLOP/s, 24 ragged requests 96
+// us = 0.48 PFLOP/s (43, 47 and 28 %).
 #pragma once
 #include "attn_kernel.cuh"
 #include "paged.cuh"

@@ -12,12 +12,15 @@
 // CTA-wide barriers to a kernel that issues in 30 % of its cycles.
 //
 // Blocks of 16 keys and 192 KB of ring per multiprocessor (8 warps x 3 blocks x 8 KB at D =
-// 128) keep some 128 KB in flight.  Measured: 64 requests of up to 8000 tokens (998 MB) 158 us
-// = 6.3 TB/s, 0.97 of a plain copy's rate; 4 of up to 131071 tokens (1.89 GB) 279 us = 6.8 TB/s;
-// 128 requests under a window of 1024 and 4 sinks (541 MB) 93 us = 5.8 TB/s: 65 blocks a unit,
-// and 2300 cycles to begin one and as many to fill its ring.  A single request of 1000 tokens:
-// 8.5 us on the GPU with the join; the chain share -> table -> keys -> partial result -> join
-// bounds it.  Times move by 3 % from one GPU to another.
+// 128) keep some 128 KB in flight.  Measured (the least and the most of several GPUs): 64
+// requests of up to 8000 tokens (998 MB) 158-168 us = 5.9-6.3 TB/s, 0.91-0.97 of a plain copy's
+// rate; 4 of up to 131071 tokens (1.89 GB) 279-291 us = 6.5-6.8 TB/s; 128 requests under a window
+// of 1024 and 4 sinks (541 MB) 93-101 us = 5.3-5.8 TB/s: 65 blocks a unit, and 2300 cycles to
+// begin one and as many to fill its ring.  That is what bounds units of few blocks: the ring
+// drains at every unit's end, and the next one's lengths, table entries, q and first blocks
+// are read one after another (500 requests of 20-200 tokens 51 us, of D = 64 47 us, where their
+// bytes take 36 and 18 us).  A single request of 1000 tokens: 8.9 us on the GPU with the join; the
+// chain share -> table -> keys -> partial result -> join bounds it.
 #include "paged.cuh"
 
 namespace pa {

@@ -33,8 +33,10 @@ __device__ __forceinline__ int unit_rows_used(const Params& P, const Config& c, 
 
 // One CTA: the cost of every request, their running sum, and for each share the unit and
 // block where it begins.  A request of many units is added up, and searched, by a whole
-// warp.  Once per step, not per layer: 5.4 us for one request, 9.1 us for 32; latency of
-// dependent steps bounds it (lengths, sums, searches), not what it reads.
+// warp.  Once per step, not per layer: 5.4-6.1 us for one token of one request, 9.1-10.8 us of
+// 32 to 500, 25 us for 8 chunks of 1000 tokens and 28-36 us for one of 4096 (128 units a key
+// head, gone through by the warps of their shares once more each); latency of dependent steps
+// bounds it (lengths, sums, searches), not what it reads.
 __global__ void __launch_bounds__(kPlanThreads)
 paged_plan_kernel(const __grid_constant__ Params P, Config c, PlanView pv) {
   __shared__ long long warp_sum[kPlanThreads / 32];

@@ -10,7 +10,7 @@
 // and every CTA scans all the lengths itself (two 4-byte loads per request, from L2) instead of
 // waiting for another one's sums; then each new token and each new page finds its
 // request by bisection in shared memory, and computes its own page from the free list
-// rather than read a table entry that another CTA writes.  3.4 us on the GPU for 8 requests
+// rather than read a table entry that another CTA writes.  3.6 us on the GPU for 8 requests
 // of one token, launch included, in a captured graph; 1000 requests with 65313 tokens take
 // 13.5 us a call, which is the host's side of it.
 #include "paged.cuh"

@@ -112,7 +112,8 @@ def make_step(block_table, old_lens, new_lens, free_pages, free_head, *, page_si
     ``PagedStep`` of the same sizes) is filled instead of a new one; none of its tensors may
     be an argument too (the next step's ``old_lens`` is this one's ``seq_lens``: use two
     in turn).  All arguments are int32 tensors on one CUDA device; at most
-    16384 requests."""
+    16384 requests, of at most 2**31 - 1 tokens each (those behind have no slot and no
+    position)."""
     B, width, row = _table(block_table, "make_step")
     dev = block_table.get_device()
     if tokens < 0:
