@@ -363,7 +363,8 @@ PA_API int pa_paged_append(const pa_paged_append_args* args, pa_stream_t stream)
  * O = 0, LSE = -inf.  Keys on table entries outside [0, pages) do not count; cache rows
  * that the mask keeps from a token, or behind a request's last token, take no part in the
  * token's result whatever they hold.  Rows of o and lse that belong to no request are
- * not written.  o and lse overlap neither each other nor any input. */
+ * not written.  o may be q itself, by the same strides; but for that, o and lse overlap neither
+ * each other nor any input. */
 typedef struct pa_paged_attn_args {
   const void* q;
   const void* k_cache;

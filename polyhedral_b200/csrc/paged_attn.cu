@@ -42,9 +42,11 @@ int check_args(const pa_paged_attn_args* a, const char* who) {
                                a->o_head_stride};
   for (long long s : strides)
     PA_CHECK_ARG(s >= 0 && s % 8 == 0, "%s: strides must be multiples of 8 elements", who);
-  // a row whose result is not finite is computed again from its q after its o was written
-  PA_CHECK_ARG(a->o != a->q && a->o != a->k_cache && a->o != a->v_cache,
-               "%s: o must not overlap q or the caches", who);
+  // a row's o is written when its q is read no more, and nothing else is then where o is q
+  PA_CHECK_ARG(a->o != a->q || (a->o_token_stride == a->q_token_stride &&
+                                a->o_head_stride == a->q_head_stride),
+               "%s: o lies over q with other strides", who);
+  PA_CHECK_ARG(a->o != a->k_cache && a->o != a->v_cache, "%s: o lies over a cache", who);
   return PA_OK;
 }
 

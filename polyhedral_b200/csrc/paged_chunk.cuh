@@ -39,6 +39,7 @@
 // share where units are short: 8 chunks of 1000 over 2000 0.64 PFLOP/s, 24 ragged requests 96
 // us = 0.48 PFLOP/s (43, 47 and 28 %).
 #pragma once
+#include <type_traits>
 #include "attn_kernel.cuh"
 #include "paged.cuh"
 
@@ -182,7 +183,9 @@ __device__ __forceinline__ constexpr bool on_fma(int pair) {
   return D == 64 && (pair & 3) == 3;
 }
 
-template <int D, bool kBf16>
+// kInPlace: o is q.  (A kernel of its own: the extra pass at a unit's end, tested at run time,
+// cost every call: 24 ragged requests took 96.5 us instead of 94.8.)
+template <int D, bool kBf16, bool kInPlace>
 __global__ void __launch_bounds__(kChunkThreads, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ ChunkParams C,
@@ -796,77 +799,84 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       // every thread writes its row, 32 bytes (a whole sector) at a time where rows are so
       // aligned
       const float inv_l = part ? 1.f : l > 0.f ? 1.f / l : 0.f;
-      float probe[4] = {l * 0.f, 0.f, 0.f, 0.f};        // 0 unless something is not finite
+      // where o is q, rows that are computed again from their q come first: a pass that only
+      // looks for them
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t r[32];
-        if (any) {
-          tmem_ld32(tO + c * 32, r);
-          tmem_wait_ld();
-          tmem_regs_ready(r);
-        } else {
-#pragma unroll
-          for (int x = 0; x < 32; ++x) r[x] = 0u;
-        }
-#pragma unroll
-        for (int x = 0; x < 32; x += 4) {
-          attn::fma2v(probe[0], probe[1], __uint_as_float(r[x]), __uint_as_float(r[x + 1]), 0.f, 0.f,
-                      probe[0], probe[1]);
-          attn::fma2v(probe[2], probe[3], __uint_as_float(r[x + 2]), __uint_as_float(r[x + 3]), 0.f,
-                      0.f, probe[2], probe[3]);
-        }
-        if (row_ptr) {
-          char* dst = reinterpret_cast<char*>(row_ptr);
-          if (part) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              st32(dst + c * 128 + x * 32, true, r[8 * x], r[8 * x + 1], r[8 * x + 2], r[8 * x + 3],
-                   r[8 * x + 4], r[8 * x + 5], r[8 * x + 6], r[8 * x + 7]);
+      for (int pass = kInPlace ? 0 : 1; pass < 2; ++pass) {
+        float probe[4] = {l * 0.f, 0.f, 0.f, 0.f};        // 0 unless something is not finite
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t r[32];
+          if (any) {
+            tmem_ld32(tO + c * 32, r);
+            tmem_wait_ld();
+            tmem_regs_ready(r);
           } else {
 #pragma unroll
-            for (int x = 0; x < 16; ++x)
-              r[x] = pack_pair<kBf16>(__uint_as_float(r[2 * x]) * inv_l,
-                                      __uint_as_float(r[2 * x + 1]) * inv_l);
+            for (int x = 0; x < 32; ++x) r[x] = 0u;
+          }
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-              st32(dst + c * 64 + x * 32, C.o32, r[8 * x], r[8 * x + 1], r[8 * x + 2], r[8 * x + 3],
-                   r[8 * x + 4], r[8 * x + 5], r[8 * x + 6], r[8 * x + 7]);
+          for (int x = 0; x < 32; x += 4) {
+            attn::fma2v(probe[0], probe[1], __uint_as_float(r[x]), __uint_as_float(r[x + 1]), 0.f, 0.f,
+                        probe[0], probe[1]);
+            attn::fma2v(probe[2], probe[3], __uint_as_float(r[x + 2]), __uint_as_float(r[x + 3]), 0.f,
+                        0.f, probe[2], probe[3]);
+          }
+          if (row_ptr && pass > 0) {
+            char* dst = reinterpret_cast<char*>(row_ptr);
+            if (part) {
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                st32(dst + c * 128 + x * 32, true, r[8 * x], r[8 * x + 1], r[8 * x + 2], r[8 * x + 3],
+                     r[8 * x + 4], r[8 * x + 5], r[8 * x + 6], r[8 * x + 7]);
+            } else {
+#pragma unroll
+              for (int x = 0; x < 16; ++x)
+                r[x] = pack_pair<kBf16>(__uint_as_float(r[2 * x]) * inv_l,
+                                        __uint_as_float(r[2 * x + 1]) * inv_l);
+#pragma unroll
+              for (int x = 0; x < 2; ++x)
+                st32(dst + c * 64 + x * 32, C.o32, r[8 * x], r[8 * x + 1], r[8 * x + 2], r[8 * x + 3],
+                     r[8 * x + 4], r[8 * x + 5], r[8 * x + 6], r[8 * x + 7]);
+            }
           }
         }
-      }
-      if (any) tc_fence_before();
-      // a value that is not finite, seen or weighed by 0: those rows key by key instead
-      uint32_t odd = __ballot_sync(0xffffffffu, valid && !((probe[0] + probe[1]) + (probe[2] + probe[3]) == 0.f));
-      if (odd) {
-        __syncwarp();
-        if (lane == 0) atomicAdd(s_slow, 1);          // the other warps' waits hold on
-      }
-      const bool slow = odd != 0;
-      for (; odd; odd &= odd - 1) {
-        const int src = __ffs(odd) - 1;
-        const int t2 = __shfl_sync(0xffffffffu, t, src), g2 = __shfl_sync(0xffffffffu, qh, src);
-        const int i2 = __shfl_sync(0xffffffffu, i, src);
-        const unsigned long long dst = __shfl_sync(0xffffffffu, row_ptr, src);
-        float m2, l2, acc[D / 32];
-        row_by_key<D, kBf16, 128>(P, u.b, u.h, t2, g2, i2, u.runs, u.blk0, u.blk1, m2, l2, acc);
-        if (lane == src) {
-          m_used = m2;
-          l = l2;
+        if (any) tc_fence_before();
+        // a value that is not finite, seen or weighed by 0: those rows key by key instead
+        const bool mine = row_ptr && !((probe[0] + probe[1]) + (probe[2] + probe[3]) == 0.f);
+        uint32_t odd = __ballot_sync(0xffffffffu, mine);
+        if (odd) {
+          __syncwarp();
+          if (lane == 0) atomicAdd(s_slow, 1);          // the other warps' waits hold on
         }
-        const float inv = part ? 1.f : l2 == 0.f ? 0.f : 1.f / l2;
+        const bool slow = odd != 0;
+        for (; odd; odd &= odd - 1) {
+          const int src = __ffs(odd) - 1;
+          const int t2 = __shfl_sync(0xffffffffu, t, src), g2 = __shfl_sync(0xffffffffu, qh, src);
+          const int i2 = __shfl_sync(0xffffffffu, i, src);
+          const unsigned long long dst = __shfl_sync(0xffffffffu, row_ptr, src);
+          float m2, l2, acc[D / 32];
+          row_by_key<D, kBf16, 128>(P, u.b, u.h, t2, g2, i2, u.runs, u.blk0, u.blk1, m2, l2, acc);
+          if (lane == src) {
+            m_used = m2;
+            l = l2;
+          }
+          const float inv = part ? 1.f : l2 == 0.f ? 0.f : 1.f / l2;
 #pragma unroll
-        for (int e = 0; e < D / 32; e += 2) {
-          if (part) {
-            float* d = reinterpret_cast<float*>(dst) + lane * (D / 32) + e;
-            d[0] = acc[e];
-            d[1] = acc[e + 1];
-          } else {
-            reinterpret_cast<uint32_t*>(dst)[lane * (D / 64) + e / 2] =
-                pack_pair<kBf16>(acc[e] * inv, acc[e + 1] * inv);
+          for (int e = 0; e < D / 32; e += 2) {
+            if (part) {
+              float* d = reinterpret_cast<float*>(dst) + lane * (D / 32) + e;
+              d[0] = acc[e];
+              d[1] = acc[e + 1];
+            } else {
+              reinterpret_cast<uint32_t*>(dst)[lane * (D / 64) + e / 2] =
+                  pack_pair<kBf16>(acc[e] * inv, acc[e + 1] * inv);
+            }
           }
         }
+        if (slow && lane == 0) atomicSub(s_slow, 1);
+        if (kInPlace && mine) row_ptr = 0;             // its row is written
       }
-      if (slow && lane == 0) atomicSub(s_slow, 1);
       if (valid) {
         if (part)
           *reinterpret_cast<float2*>(part + (size_t)256 * D + 2 * rr) = make_float2(m_used, l);
@@ -899,11 +909,14 @@ int launch_chunk_body(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
                       const ChunkParams& C, const PlanView& pv, float* scratch, int sms,
                       cudaStream_t stream) {
   constexpr int kMinRegs = (256 * kChunkSoftRegs + 128 * kChunkOtherRegs) / kChunkThreads;
-  const int rc = prepare_kernel<paged_chunk_kernel<D, kBf16>>("pa_paged_attn", ChunkSmem<D>::kAlloc,
-                                                              kMinRegs);
-  if (rc) return rc;
-  return launch_after("pa_paged_attn", paged_chunk_kernel<D, kBf16>, sms, kChunkThreads,
-                      ChunkSmem<D>::kAlloc, stream, tq, tk, tv, C, pv.shares, pv.meta, scratch);
+  auto go = [&](auto in_place) {
+    constexpr auto kKernel = paged_chunk_kernel<D, kBf16, decltype(in_place)::value>;
+    const int rc = prepare_kernel<kKernel>("pa_paged_attn", ChunkSmem<D>::kAlloc, kMinRegs);
+    if (rc) return rc;
+    return launch_after("pa_paged_attn", kKernel, sms, kChunkThreads, ChunkSmem<D>::kAlloc, stream, tq,
+                        tk, tv, C, pv.shares, pv.meta, scratch);
+  };
+  return C.p.o == C.p.q ? go(std::true_type{}) : go(std::false_type{});
 }
 
 }  // namespace paged

@@ -265,7 +265,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, q_start, kind, p
     ``plan`` is ``make_plan``'s for these lengths and this mask; without one it is built
     first (``max_new`` / ``max_len`` as there).  The plan of another step gives wrong results
     and is reported: ``check`` or ``plan.status()`` shows it.  ``out`` / ``lse_out`` are written
-    in place of new tensors and overlap no input (``out`` may not be ``q``).  ``check``
+    in place of new tensors and overlap no input; but ``out`` may be ``q``.  ``check``
     synchronises and raises if the kernel reported a failure."""
     if q.dim() != 3:
         raise ValueError("q must be [tokens, heads, D]")

@@ -7,16 +7,17 @@ from polyhedral_b200 import _lib
 from tests.test_paged_host import PTR, _attn_args, lib  # noqa: F401
 
 
-@pytest.mark.parametrize("field", ["q", "k_cache", "v_cache"])
-def test_results_over_the_inputs(lib, field):  # noqa: F811
+@pytest.mark.parametrize("field,word", [("q", b"over q with other strides"), ("k_cache", b"over a cache"),
+                                        ("v_cache", b"over a cache")])
+def test_results_over_the_inputs(lib, field, word):  # noqa: F811
     a = _attn_args()
-    a.o = 4096
+    a.o, a.o_token_stride = 4096, 128
     setattr(a, field, 4096)
     for call in (lambda: lib.pa_paged_attn(ctypes.byref(a), PTR, 1 << 30, PTR, 1 << 40, None),
                  lambda: lib.pa_paged_attn_withheld(ctypes.byref(a), PTR, 1 << 30, PTR, 1 << 40,
                                                     2_000_000, None)):
         assert call() == _lib.PA_ERR_ARG
-        assert b"o must not overlap" in lib.pa_last_error()
+        assert word in lib.pa_last_error()
 
 
 @pytest.mark.parametrize("limit", [0, -1, 999, 10**9 + 1])
