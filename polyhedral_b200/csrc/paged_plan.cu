@@ -258,6 +258,9 @@ paged_plan_kernel(const __grid_constant__ Params P, Config c, PlanView pv) {
 // the warps of a CTA share a row's.  (The order of `cuts` is that of an atomic counter; it
 // decides only which warp joins which row.)
 constexpr int kJoinWarps = 8;
+__host__ __device__ inline int check_ctas(const Config& c) {   // a thread per share
+  return (c.workers + kJoinWarps * 32 - 1) / (kJoinWarps * 32);
+}
 
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kJoinWarps * 32)
@@ -270,11 +273,13 @@ paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
   pdl_wait();
   pdl_begin_next();
   const int used = pv.meta[0], cuts = pv.meta[1], rows = pv.meta[2];
-  // the plan's lengths, by the last CTAs, which have no row where the work is little
-  {
-    const int x = (gridDim.x - 1 - blockIdx.x) * (kJoinWarps * 32) + threadIdx.x;
-    if (other_lengths(P, pv.shares, used, x, gridDim.x * kJoinWarps * 32))
+  // CTAs behind those that join compare the plan's lengths (the joining ones would begin later)
+  const int ctas = gridDim.x - check_ctas(c);
+  if ((int)blockIdx.x >= ctas) {
+    if (other_lengths(P, pv.shares, used, (blockIdx.x - ctas) * (kJoinWarps * 32) + threadIdx.x,
+                      check_ctas(c) * (kJoinWarps * 32)))
       atomicExch(pv.status, (int32_t)DEV_OTHER_LENGTHS);
+    return;
   }
   const bool many = used > kJoinWarps * cuts;   // pieces per unit, on average
   const int unit_rows = c.unit_rows;
@@ -322,7 +327,7 @@ paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
   if (!many && c.half_tokens) {
     constexpr int kGroup = 8;
     const int groups = (rows + kGroup - 1) / kGroup;
-    for (int it = blockIdx.x * kJoinWarps + warp; it < cuts * groups; it += gridDim.x * kJoinWarps) {
+    for (int it = blockIdx.x * kJoinWarps + warp; it < cuts * groups; it += ctas * kJoinWarps) {
       const int k = it / groups;
       const Cut cut = pv.cuts[k];
       const int r0 = (it - k * groups) * kGroup;
@@ -369,7 +374,7 @@ paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
   }
 
   const int it0 = many ? blockIdx.x : blockIdx.x * kJoinWarps + warp;
-  for (int it = it0; it < cuts * rows; it += many ? gridDim.x : gridDim.x * kJoinWarps) {
+  for (int it = it0; it < cuts * rows; it += many ? ctas : ctas * kJoinWarps) {
     const int k = it / rows, r = it - k * rows;
     const Cut cut = pv.cuts[k];
     int g;
@@ -444,7 +449,7 @@ int launch_plan(const Params& P, const Config& c, const PlanView& pv, cudaStream
 int launch_join(const Params& P, bool bf16, int D, const PlanView& pv, const Config& c,
                 const float* scratch, int sms, cudaStream_t stream) {
   auto go = [&](auto kernel) {
-    return launch_after("pa_paged_attn", kernel, sms * 4, kJoinWarps * 32, 0, stream, P, c, pv, scratch);
+    return launch_after("pa_paged_attn", kernel, sms * 4 + check_ctas(c), kJoinWarps * 32, 0, stream, P, c, pv, scratch);
   };
   if (D == 128) return bf16 ? go(paged_join_kernel<128, true>) : go(paged_join_kernel<128, false>);
   return bf16 ? go(paged_join_kernel<64, true>) : go(paged_join_kernel<64, false>);
