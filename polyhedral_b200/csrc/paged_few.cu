@@ -19,7 +19,7 @@
 // begin one and as many to fill its ring.  That is what bounds units of few blocks: the ring
 // drains at every unit's end, and the next one's lengths, table entries, q and first blocks
 // are read one after another (500 requests of 20-200 tokens 51 us, of D = 64 47 us, where their
-// bytes take 36 and 18 us).  A single request of 1000 tokens: 8.5 us on the GPU with the join; the
+// bytes take 36 and 18 us).  A single request of 1000 tokens: 8.7 us on the GPU with the join; the
 // chain share -> table -> keys -> partial result -> join bounds it.
 #include "paged.cuh"
 

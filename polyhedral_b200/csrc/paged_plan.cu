@@ -262,8 +262,10 @@ __host__ __device__ inline int check_ctas(const Config& c) {   // a thread per s
   return (c.workers + kJoinWarps * 32 - 1) / (kJoinWarps * 32);
 }
 
+// 3 CTAs a multiprocessor: 78 registers a thread, which the loads of 4 rows at once need (with
+// 64 at D = 64, 24 ragged requests took 96.2 us instead of 94.8).
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(kJoinWarps * 32)
+__global__ void __launch_bounds__(kJoinWarps * 32, 3)
 paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
                   const float* __restrict__ scratch) {
   constexpr int E = D / 32;
@@ -273,11 +275,11 @@ paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
   pdl_wait();
   pdl_begin_next();
   const int used = pv.meta[0], cuts = pv.meta[1], rows = pv.meta[2];
-  // CTAs behind those that join compare the plan's lengths (the joining ones would begin later)
-  const int ctas = gridDim.x - check_ctas(c);
-  if ((int)blockIdx.x >= ctas) {
-    if (other_lengths(P, pv.shares, used, (blockIdx.x - ctas) * (kJoinWarps * 32) + threadIdx.x,
-                      check_ctas(c) * (kJoinWarps * 32)))
+  // the first CTAs compare the plan's lengths instead of joining (a joining one would begin later)
+  const int checks = check_ctas(c), ctas = gridDim.x - checks, cta = (int)blockIdx.x - checks;
+  if (cta < 0) {
+    if (other_lengths(P, pv.shares, used, blockIdx.x * (kJoinWarps * 32) + threadIdx.x,
+                      checks * (kJoinWarps * 32)))
       atomicExch(pv.status, (int32_t)DEV_OTHER_LENGTHS);
     return;
   }
@@ -327,7 +329,7 @@ paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
   if (!many && c.half_tokens) {
     constexpr int kGroup = 8;
     const int groups = (rows + kGroup - 1) / kGroup;
-    for (int it = blockIdx.x * kJoinWarps + warp; it < cuts * groups; it += ctas * kJoinWarps) {
+    for (int it = cta * kJoinWarps + warp; it < cuts * groups; it += ctas * kJoinWarps) {
       const int k = it / groups;
       const Cut cut = pv.cuts[k];
       const int r0 = (it - k * groups) * kGroup;
@@ -373,7 +375,7 @@ paged_join_kernel(const __grid_constant__ Params P, Config c, PlanView pv,
     return;
   }
 
-  const int it0 = many ? blockIdx.x : blockIdx.x * kJoinWarps + warp;
+  const int it0 = many ? cta : cta * kJoinWarps + warp;
   for (int it = it0; it < cuts * rows; it += many ? ctas : ctas * kJoinWarps) {
     const int k = it / rows, r = it - k * rows;
     const Cut cut = pv.cuts[k];
@@ -449,7 +451,7 @@ int launch_plan(const Params& P, const Config& c, const PlanView& pv, cudaStream
 int launch_join(const Params& P, bool bf16, int D, const PlanView& pv, const Config& c,
                 const float* scratch, int sms, cudaStream_t stream) {
   auto go = [&](auto kernel) {
-    return launch_after("pa_paged_attn", kernel, sms * 4 + check_ctas(c), kJoinWarps * 32, 0, stream, P, c, pv, scratch);
+    return launch_after("pa_paged_attn", kernel, sms * 4, kJoinWarps * 32, 0, stream, P, c, pv, scratch);
   };
   if (D == 128) return bf16 ? go(paged_join_kernel<128, true>) : go(paged_join_kernel<128, false>);
   return bf16 ? go(paged_join_kernel<64, true>) : go(paged_join_kernel<64, false>);
