@@ -30,7 +30,7 @@
 // us in a short run, 1090-1140 in a long one = 1.09-1.22 PFLOP/s (of 1.64 measured for a
 // library product in a burst, 1.40 sustained: like that one it runs into the power limit, at
 // 1.55 GHz); tensor cores and exponential unit both 64 % busy.  8 chunks of 2000 under a window
-// of 1024 and 4 sinks, a key head per query head: 450-496 us = 0.54-0.60 PFLOP/s of live products;
+// of 1024 and 4 sinks, a key head per query head: 450-501 us = 0.54-0.60 PFLOP/s of live products;
 // a unit has 11 super-tiles, one of them for the 4 sinks, 4 of a half's 10 are partly masked
 // and its first and last are the other half's, and between units nothing overlaps a half's
 // last products, result and first scores (7 000 of its 45 000 cycles).  D = 64: no unit is
